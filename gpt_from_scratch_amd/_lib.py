@@ -29,7 +29,10 @@ EXPORTED = ("mi_version", "mi_status_str", "mi_last_error", "mi_attn_fwd", "mi_a
             "mi_adamw_workspace", "mi_grad_sumsq", "mi_adamw_step", "mi_attn_bwd_noalloc",
             "mi_rmsnorm_add_fwd", "mi_rmsnorm_add_bwd", "mi_attn_bwd_rope",
             "mi_rmsnorm_bwd_acc", "mi_rmsnorm_add_bwd_acc", "mi_copy_qk",
-            "mi_wgrad_workspace", "mi_wgrad_suits", "mi_wgrad")
+            "mi_wgrad_workspace", "mi_wgrad_suits", "mi_wgrad",
+            "mi_rotary_qk", "mi_qk_norm_rotary", "mi_qk_norm_rotary_workspace",
+            "mi_qk_norm_rotary_bwd", "mi_sattn_tiles", "mi_sattn_fwd", "mi_sattn_bwd_workspace",
+            "mi_sattn_bwd", "mi_decode_workspace", "mi_decode_attn")
 
 # B*H*S limit of mi_attn_bwd_noalloc (its static workspace array), include/mi_attn.h
 NOALLOC_MAX_ROWS = 1 << 20
@@ -39,6 +42,24 @@ _lib = None
 
 class MiError(RuntimeError):
     """A non-OK status returned by the C ABI."""
+
+
+class Rotary(ctypes.Structure):
+    """mi_rotary."""
+    _fields_ = [("tab_dtype", ctypes.c_int), ("S", ctypes.c_int), ("B", ctypes.c_int),
+                ("H", ctypes.c_int), ("Hk", ctypes.c_int), ("D", ctypes.c_int),
+                ("R", ctypes.c_int), ("interleaved", ctypes.c_int),
+                ("cos_tab", ctypes.c_void_p), ("sin_tab", ctypes.c_void_p),
+                ("cos_strides", ctypes.c_int64 * 2), ("sin_strides", ctypes.c_int64 * 2),
+                ("table_rows", ctypes.c_int64), ("positions", ctypes.c_void_p),
+                ("pos_strides", ctypes.c_int64 * 2), ("pos_bytes", ctypes.c_int)]
+
+
+class ScoreMods(ctypes.Structure):
+    """mi_score_mods."""
+    _fields_ = [("causal", ctypes.c_int), ("softcap", ctypes.c_float),
+                ("slopes", ctypes.c_void_p), ("document_ids", ctypes.c_void_p),
+                ("prefix_lens", ctypes.c_void_p)]
 
 
 def _i64x4():
@@ -115,6 +136,29 @@ def _declare(lib):
     lib.mi_wgrad_suits.argtypes = [i64, i64, i64]
     lib.mi_wgrad.restype = i
     lib.mi_wgrad.argtypes = [i, i64, i64, i64, p, i64, p, i64, p, i, p, i64, p]
+    how, mods = ctypes.POINTER(Rotary), ctypes.POINTER(ScoreMods)
+    lib.mi_rotary_qk.restype = i
+    lib.mi_rotary_qk.argtypes = [i, how, i, p, i64p, p, i64p, p, i64p, p, i64p, p]
+    lib.mi_qk_norm_rotary.restype = i
+    lib.mi_qk_norm_rotary.argtypes = [i, i, how, f, p, i64p, p, i64p, p, p, p, i64p, p, i64p, p]
+    lib.mi_qk_norm_rotary_workspace.restype = i64
+    lib.mi_qk_norm_rotary_workspace.argtypes = [how]
+    lib.mi_qk_norm_rotary_bwd.restype = i
+    lib.mi_qk_norm_rotary_bwd.argtypes = [i, i, how, f, p, i64p, p, i64p, p, p, p, i64p, p, i64p,
+                                          p, i64p, p, i64p, p, p, p, i64, p]
+    lib.mi_sattn_tiles.restype = i64
+    lib.mi_sattn_tiles.argtypes = [i, i, i]
+    lib.mi_sattn_fwd.restype = i
+    lib.mi_sattn_fwd.argtypes = [i] * 7 + [f, mods, p, i64p, p, i64p, p, i64p, p, i64p, p, p, p]
+    lib.mi_sattn_bwd_workspace.restype = i64
+    lib.mi_sattn_bwd_workspace.argtypes = [i] * 7
+    lib.mi_sattn_bwd.restype = i
+    lib.mi_sattn_bwd.argtypes = [i] * 7 + [f, mods] + [p, i64p] * 5 + [p, p, p, i64] + \
+        [p, i64p] * 3 + [p]
+    lib.mi_decode_workspace.restype = i64
+    lib.mi_decode_workspace.argtypes = [i] * 6
+    lib.mi_decode_attn.restype = i
+    lib.mi_decode_attn.argtypes = [i] * 6 + [f, f, p, p] + [p, i64p] * 4 + [p, i64, p]
     lib.mi_adamw_workspace.restype = i64
     lib.mi_adamw_workspace.argtypes = []
     lib.mi_grad_sumsq.restype = i
@@ -488,6 +532,139 @@ def wgrad(dy, x, dweight=None):
     if acc:
         torch.autograd.graph.increment_version(dweight)  # as addmm_ would
     return dweight
+
+
+def _rotary_how(q, k, cos, sin, positions, interleaved):
+    """mi_rotary for q [S, B, H, D] and k [S, B, Hk, D], whose tables and positions
+    the caller has checked."""
+    S, B, H, D = q.shape
+    how = Rotary(dtype_code(cos), S, B, H, k.shape[2], D, 2 * cos.shape[1], int(interleaved),
+                 cos.data_ptr(), sin.data_ptr(), cos.stride(), sin.stride(), cos.shape[0])
+    if positions is not None:
+        how.positions = positions.data_ptr()
+        how.pos_strides = (positions.stride(0), positions.stride(1) if positions.dim() == 2 else 0)
+        how.pos_bytes = positions.element_size()
+    return how
+
+
+def rotary_qk(q, k, cos, sin, positions, interleaved: bool, q_out, k_out, inverse: bool):
+    """Enqueue the rotation of q [S, B, H, D] and k [S, B, Hk, D]."""
+    _require_gpu(q, k, cos, sin, q_out, k_out, *([] if positions is None else [positions]))
+    how = _rotary_how(q, k, cos, sin, positions, interleaved)
+    st = lib().mi_rotary_qk(dtype_code(q), how, int(inverse), _ptr(q), _strides(q, 4), _ptr(k),
+                            _strides(k, 4), _ptr(q_out), _strides(q_out, 4), _ptr(k_out),
+                            _strides(k_out, 4), _stream(q))
+    _check(st, "mi_rotary_qk")
+
+
+def qk_norm_rotary(q, k, wq, wk, cos, sin, positions, interleaved: bool, eps: float, q_out, k_out):
+    """Enqueue norm and rotation of q and k; wq, wk dense [D]."""
+    _require_gpu(q, k, wq, wk, cos, sin, q_out, k_out, *([] if positions is None else [positions]))
+    how = _rotary_how(q, k, cos, sin, positions, interleaved)
+    st = lib().mi_qk_norm_rotary(dtype_code(q), dtype_code(wq), how, float(eps), _ptr(q),
+                                 _strides(q, 4), _ptr(k), _strides(k, 4), _ptr(wq), _ptr(wk),
+                                 _ptr(q_out), _strides(q_out, 4), _ptr(k_out), _strides(k_out, 4),
+                                 _stream(q))
+    _check(st, "mi_qk_norm_rotary")
+
+
+def qk_norm_rotary_bwd(q, k, wq, wk, cos, sin, positions, interleaved: bool, eps: float, gq, gk,
+                       dq, dk, dwq, dwk):
+    """Enqueue the backward of qk_norm_rotary: dq, dk, dwq, dwk from gq, gk."""
+    _require_gpu(q, k, wq, wk, cos, sin, gq, gk, dq, dk, dwq, dwk,
+                 *([] if positions is None else [positions]))
+    how = _rotary_how(q, k, cos, sin, positions, interleaved)
+    n = lib().mi_qk_norm_rotary_workspace(how)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device)
+    st = lib().mi_qk_norm_rotary_bwd(dtype_code(q), dtype_code(wq), how, float(eps), _ptr(q),
+                                     _strides(q, 4), _ptr(k), _strides(k, 4), _ptr(wq), _ptr(wk),
+                                     _ptr(gq), _strides(gq, 4), _ptr(gk), _strides(gk, 4),
+                                     _ptr(dq), _strides(dq, 4), _ptr(dk), _strides(dk, 4),
+                                     _ptr(dwq), _ptr(dwk), _ptr(ws), n, _stream(q))
+    _check(st, "mi_qk_norm_rotary_bwd")
+
+
+def _row_strides(t: torch.Tensor):
+    """t's strides, those of size-1 dims (which address nothing) as 0."""
+    last = t.dim() - 1
+    return (ctypes.c_int64 * t.dim())(*(0 if n == 1 and d < last else s
+                                        for d, (n, s) in enumerate(zip(t.shape, t.stride()))))
+
+
+def rows_ready(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy whose rows over the last dim have unit stride and are 16-byte
+    aligned and less than 8 MB apart, as the kernels of attention with modified
+    scores read them."""
+    e = t.element_size()
+    st = list(_row_strides(t))[:-1]
+    ok = t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and not any(s * e % 16 for s in st) \
+        and st[-1] * e * 256 < 1 << 31
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _opt_ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _score_mods(causal, softcap, slopes, docs, prefix):
+    return ScoreMods(int(causal), float(softcap or 0.0), _opt_ptr(slopes), _opt_ptr(docs),
+                     _opt_ptr(prefix))
+
+
+def sattn_tiles(q, k) -> int:
+    return int(lib().mi_sattn_tiles(q.shape[0], q.shape[2], k.shape[2]))
+
+
+def sattn_fwd(q, k, v, mods, scale: float):
+    """Enqueue attention with modified scores: (o, lse, tiles) of q [B, H, Sq, D] and
+    k, v [B, Hk, Sk, D] by rows_ready; mods = (causal, softcap, slopes, docs, prefix),
+    dense tensors or None."""
+    _require_gpu(q, k, v, *(t for t in mods[2:] if t is not None))
+    (B, H, Sq, D), (_, Hk, Sk, _) = q.shape, k.shape
+    o = torch.empty(B, H, Sq, D, dtype=q.dtype, device=q.device)
+    lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device)
+    tiles = None
+    if mods[3] is not None:
+        tiles = torch.empty(sattn_tiles(q, k), dtype=torch.int32, device=q.device)
+    st = lib().mi_sattn_fwd(dtype_code(q), B, H, Hk, Sq, Sk, D, float(scale), _score_mods(*mods),
+                            _ptr(q), _row_strides(q), _ptr(k), _row_strides(k), _ptr(v),
+                            _row_strides(v), _ptr(o), _row_strides(o), _ptr(lse), _opt_ptr(tiles),
+                            _stream(q))
+    _check(st, "mi_sattn_fwd")
+    return o, lse, tiles
+
+
+def sattn_bwd(q, k, v, o, do, lse, tiles, mods, scale: float):
+    """Enqueue the backward of sattn_fwd: (dq, dk, dv)."""
+    _require_gpu(q, k, v, o, do, lse, *(t for t in mods[2:] if t is not None))
+    (B, H, Sq, D), (_, Hk, Sk, _) = q.shape, k.shape
+    n = lib().mi_sattn_bwd_workspace(dtype_code(q), B, H, Hk, Sq, Sk, D)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device)
+    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
+    st = lib().mi_sattn_bwd(dtype_code(q), B, H, Hk, Sq, Sk, D, float(scale), _score_mods(*mods),
+                            _ptr(q), _row_strides(q), _ptr(k), _row_strides(k), _ptr(v),
+                            _row_strides(v), _ptr(o), _row_strides(o), _ptr(do), _row_strides(do),
+                            _ptr(lse), _opt_ptr(tiles), _ptr(ws), n, _ptr(dq), _row_strides(dq),
+                            _ptr(dk), _row_strides(dk), _ptr(dv), _row_strides(dv), _stream(q))
+    _check(st, "mi_sattn_bwd")
+    return dq, dk, dv
+
+
+def decode_attn(q, k, v, lengths, softcap, slopes, scale: float):
+    """Enqueue attention of one token q [B, H, D] of each sequence over its cache
+    k, v [B, Hk, S, D]; returns o."""
+    _require_gpu(q, k, v, *(t for t in (lengths, slopes) if t is not None))
+    (B, H, D), (_, Hk, S, _) = q.shape, k.shape
+    o = torch.empty(B, H, D, dtype=q.dtype, device=q.device)
+    n = lib().mi_decode_workspace(dtype_code(q), B, H, Hk, S, D)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
+    st = lib().mi_decode_attn(dtype_code(q), B, H, Hk, S, D, float(scale), float(softcap or 0.0),
+                              _opt_ptr(slopes), _opt_ptr(lengths), _ptr(q), _row_strides(q),
+                              _ptr(k), _row_strides(k), _ptr(v), _row_strides(v), _ptr(o),
+                              _row_strides(o), _opt_ptr(ws), n, _stream(q))
+    _check(st, "mi_decode_attn")
+    return o
 
 
 def adamw_workspace() -> int:

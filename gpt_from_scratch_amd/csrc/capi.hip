@@ -23,6 +23,7 @@
 
 #include "../../include/mi_attn.h"
 #include "mi_kernels.h"
+#include "sattn_device.h"
 
 namespace {
 
@@ -171,7 +172,7 @@ mi::AttnArgs grad_args(int B, int H, int S, int D, int causal, float scale, cons
 
 extern "C" {
 
-int mi_version(void) { return (2 << 16) | 5; }
+int mi_version(void) { return (2 << 16) | 6; }
 
 const char* mi_status_str(mi_status s) {
   switch (s) {
@@ -1132,3 +1133,390 @@ extern "C" mi_status mi_attn_bwd_noalloc(
                      o, o_strides, dout, dout_strides, lse, ws, dq, dq_strides, dk, dk_strides,
                      dv, dv_strides, stream);
 }
+
+// ---------------------------------------------------------------------------
+// Rotary embedding at given positions, with the norm of each head in front
+// ---------------------------------------------------------------------------
+namespace {
+
+mi_status check_rotary(mi_dtype dtype, const mi_rotary* how) {
+  if (how == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "how: null pointer");
+  if (!dtype_ok(dtype) || !dtype_ok(how->tab_dtype))
+    return fail(MI_ERR_INVALID_ARGUMENT, "unknown dtype");
+  if (how->S <= 0 || how->B <= 0 || how->H <= 0 || how->Hk <= 0 || how->D <= 0)
+    return fail(MI_ERR_INVALID_ARGUMENT, "sizes must be positive (S=%d B=%d H=%d Hk=%d D=%d)",
+                how->S, how->B, how->H, how->Hk, how->D);
+  if (how->R < 2 || how->R % 2 || how->R > how->D)
+    return fail(MI_ERR_INVALID_ARGUMENT, "R = %d: an even number from 2 to D = %d", how->R, how->D);
+  // 32-bit row and element counts inside the kernels
+  if (how->D > (1 << 16) || how->H > (1 << 24) || how->Hk > (1 << 24) ||
+      (double)how->S * how->B * ((double)how->H + how->Hk) >= 2147483648.0)
+    return fail(MI_ERR_UNSUPPORTED, "tensor too large for one launch");
+  if (!how->cos_tab || !how->sin_tab)
+    return fail(MI_ERR_INVALID_ARGUMENT, "cos/sin: null pointer");
+  if (how->table_rows <= 0 || (how->positions == nullptr && how->table_rows < how->S))
+    return fail(MI_ERR_INVALID_ARGUMENT, "%lld table rows for %d positions",
+                (long long)how->table_rows, how->S);
+  if (how->positions && how->pos_bytes != 4 && how->pos_bytes != 8)
+    return fail(MI_ERR_INVALID_ARGUMENT, "positions of %d bytes: 4 or 8", how->pos_bytes);
+  return MI_OK;
+}
+
+// Whether [S, B, heads, D] rows are whole 16-byte chunks in place.
+bool rows16(const void* p, const int64_t* st, int esz) {
+  return ((uintptr_t)p) % 16 == 0 && st[3] == 1 && st[0] * esz % 16 == 0 &&
+         st[1] * esz % 16 == 0 && st[2] * esz % 16 == 0;
+}
+
+// The argument block; `vec` becomes whether the vector kernels can run it.
+mi::RotaryArgs rotary_args(mi_dtype dtype, const mi_rotary& h, const void* const (&x)[2],
+                           const int64_t* const (&xs)[2], void* const (&out)[2],
+                           const int64_t* const (&os)[2], bool& vec) {
+  mi::RotaryArgs a = {};
+  a.cos = h.cos_tab;
+  a.sin = h.sin_tab;
+  a.cs_s = h.cos_strides[0]; a.cs_i = h.cos_strides[1];
+  a.ss_s = h.sin_strides[0]; a.ss_i = h.sin_strides[1];
+  a.T = h.table_rows;
+  a.pos = h.positions;
+  a.pos_ss = h.pos_strides[0];
+  a.pos_sb = h.pos_strides[1];
+  a.pos64 = h.pos_bytes == 8;
+  a.tab_dt = h.tab_dtype;
+  a.S = h.S; a.B = h.B; a.D = h.D; a.R = h.R;
+  a.interleaved = h.interleaved ? 1 : 0;
+  const int esz = elem_size(dtype), n = 16 / esz;
+  // a lane's n angles come with aligned loads: 16 bytes, or all n of them if less
+  const int tsz = elem_size(h.tab_dtype), ab = n * tsz < 16 ? n * tsz : 16;
+  vec = mi::rotary_vec_ok(dtype, h.D, h.R) && a.cs_i == 1 && a.ss_i == 1 &&
+        a.cs_s * tsz % ab == 0 && a.ss_s * tsz % ab == 0 && ((uintptr_t)a.cos) % ab == 0 &&
+        ((uintptr_t)a.sin) % ab == 0;
+  for (int i = 0; i < 2; ++i) {
+    mi::RotaryTensor& t = a.t[i];
+    t.heads = i ? h.Hk : h.H;
+    t.x = x[i];
+    t.x_ss = xs[i][0]; t.x_sb = xs[i][1]; t.x_sh = xs[i][2]; t.x_sd = xs[i][3];
+    t.out = out[i];
+    t.o_ss = os[i][0]; t.o_sb = os[i][1]; t.o_sh = os[i][2]; t.o_sd = os[i][3];
+    vec = vec && rows16(x[i], xs[i], esz) && rows16(out[i], os[i], esz);
+  }
+  return a;
+}
+
+mi_status check_pointers(std::initializer_list<const void*> ps) {
+  for (const void* p : ps)
+    if (p == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "null pointer");
+  return MI_OK;
+}
+
+mi_status check_norm(mi_dtype w_dtype, const mi_rotary* how, float eps) {
+  if (!dtype_ok(w_dtype)) return fail(MI_ERR_INVALID_ARGUMENT, "unknown weight dtype %d", w_dtype);
+  if (how->D > 512) return fail(MI_ERR_UNSUPPORTED, "D = %d: at most 512 with the norm", how->D);
+  if (!(eps >= 0.f) || std::isinf(eps))
+    return fail(MI_ERR_INVALID_ARGUMENT, "eps must be finite and not negative");
+  return MI_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+mi_status mi_rotary_qk(mi_dtype dtype, const mi_rotary* how, int inverse, const void* q,
+                       const int64_t q_strides[4], const void* k, const int64_t k_strides[4],
+                       void* q_out, const int64_t q_out_strides[4], void* k_out,
+                       const int64_t k_out_strides[4], void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_rotary(dtype, how)) != MI_OK) return st;
+  if ((st = check_pointers({q, k, q_out, k_out, q_strides, k_strides, q_out_strides,
+                            k_out_strides})) != MI_OK)
+    return st;
+  bool vec;
+  mi::RotaryArgs a = rotary_args(dtype, *how, {q, k}, {q_strides, k_strides}, {q_out, k_out},
+                                 {q_out_strides, k_out_strides}, vec);
+  a.inverse = inverse ? 1 : 0;
+  return launched(mi::launch_rotary(dtype, 0, a, vec, (hipStream_t)stream), "rotary_qk");
+}
+
+mi_status mi_qk_norm_rotary(mi_dtype dtype, mi_dtype w_dtype, const mi_rotary* how, float eps,
+                            const void* q, const int64_t q_strides[4], const void* k,
+                            const int64_t k_strides[4], const void* q_weight,
+                            const void* k_weight, void* q_out, const int64_t q_out_strides[4],
+                            void* k_out, const int64_t k_out_strides[4], void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_rotary(dtype, how)) != MI_OK || (st = check_norm(w_dtype, how, eps)) != MI_OK)
+    return st;
+  if ((st = check_pointers({q, k, q_out, k_out, q_weight, k_weight, q_strides, k_strides,
+                            q_out_strides, k_out_strides})) != MI_OK)
+    return st;
+  bool vec;
+  mi::RotaryArgs a = rotary_args(dtype, *how, {q, k}, {q_strides, k_strides}, {q_out, k_out},
+                                 {q_out_strides, k_out_strides}, vec);
+  vec = vec && ((uintptr_t)q_weight) % 16 == 0 && ((uintptr_t)k_weight) % 16 == 0;
+  a.t[0].w = q_weight;
+  a.t[1].w = k_weight;
+  a.w_dt = w_dtype;
+  a.eps = eps;
+  return launched(mi::launch_rotary(dtype, 1, a, vec, (hipStream_t)stream), "qk_norm_rotary");
+}
+
+int64_t mi_qk_norm_rotary_workspace(const mi_rotary* how) {
+  if (how == nullptr || how->S <= 0 || how->B <= 0 || how->H <= 0 || how->Hk <= 0 || how->D <= 0)
+    return 0;
+  const int64_t n = (int64_t)how->S * how->B;
+  return ((int64_t)mi::rotary_grad_blocks(n * how->H) + mi::rotary_grad_blocks(n * how->Hk)) *
+         how->D;
+}
+
+mi_status mi_qk_norm_rotary_bwd(mi_dtype dtype, mi_dtype w_dtype, const mi_rotary* how, float eps,
+                                const void* q, const int64_t q_strides[4], const void* k,
+                                const int64_t k_strides[4], const void* q_weight,
+                                const void* k_weight, const void* dq_out,
+                                const int64_t dq_out_strides[4], const void* dk_out,
+                                const int64_t dk_out_strides[4], void* dq,
+                                const int64_t dq_strides[4], void* dk,
+                                const int64_t dk_strides[4], void* dq_weight, void* dk_weight,
+                                float* workspace, int64_t workspace_elems, void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_rotary(dtype, how)) != MI_OK || (st = check_norm(w_dtype, how, eps)) != MI_OK)
+    return st;
+  if ((st = check_pointers({q, k, q_weight, k_weight, dq_out, dk_out, dq, dk, dq_weight, dk_weight,
+                            workspace, q_strides, k_strides, dq_out_strides, dk_out_strides,
+                            dq_strides, dk_strides})) != MI_OK)
+    return st;
+  const int64_t want = mi_qk_norm_rotary_workspace(how);
+  if (workspace_elems < want)
+    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted",
+                (long long)workspace_elems, (long long)want);
+  bool vec;
+  mi::RotaryArgs a = rotary_args(dtype, *how, {q, k}, {q_strides, k_strides}, {dq, dk},
+                                 {dq_strides, dk_strides}, vec);
+  const int esz = elem_size(dtype);
+  vec = vec && ((uintptr_t)q_weight) % 16 == 0 && ((uintptr_t)k_weight) % 16 == 0 &&
+        rows16(dq_out, dq_out_strides, esz) && rows16(dk_out, dk_out_strides, esz);
+  const void* const dy[2] = {dq_out, dk_out};
+  const int64_t* const dys[2] = {dq_out_strides, dk_out_strides};
+  void* const dw[2] = {dq_weight, dk_weight};
+  const void* const w[2] = {q_weight, k_weight};
+  for (int i = 0; i < 2; ++i) {
+    mi::RotaryTensor& t = a.t[i];
+    t.dy = dy[i];
+    t.dy_ss = dys[i][0]; t.dy_sb = dys[i][1]; t.dy_sh = dys[i][2]; t.dy_sd = dys[i][3];
+    t.w = w[i];
+    t.dw = dw[i];
+    a.blocks[i] = mi::rotary_grad_blocks((int64_t)how->S * how->B * t.heads);
+  }
+  a.w_dt = w_dtype;
+  a.eps = eps;
+  a.part = workspace;
+  return launched(mi::launch_rotary(dtype, 2, a, vec, (hipStream_t)stream), "qk_norm_rotary_bwd");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------
+// Attention with modified scores
+// ---------------------------------------------------------------------------
+namespace {
+
+mi_status check_sattn(int dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                      float softcap) {
+  if (!dtype_ok(dtype)) return fail(MI_ERR_INVALID_ARGUMENT, "unknown dtype %d", dtype);
+  if (B <= 0 || H <= 0 || Hk <= 0 || Sq <= 0 || Sk <= 0 || D <= 0)
+    return fail(MI_ERR_INVALID_ARGUMENT,
+                "sizes must be positive (B=%d H=%d Hk=%d Sq=%d Sk=%d D=%d)", B, H, Hk, Sq, Sk, D);
+  if (H % Hk) return fail(MI_ERR_INVALID_ARGUMENT, "H = %d is no multiple of Hk = %d", H, Hk);
+  if (Sq > Sk) return fail(MI_ERR_INVALID_ARGUMENT, "more queries (%d) than keys (%d)", Sq, Sk);
+  if (D % 8 || D > 128)
+    return fail(MI_ERR_UNSUPPORTED, "head dim %d: a multiple of 8 up to 128", D);
+  // tile indexes and positions (as exact floats) keep 24 bits, rows 31
+  if (Sk > (1 << 24) || (double)B * H * Sq >= 2147483648.0 || (double)B * Hk * Sk >= 2147483648.0)
+    return fail(MI_ERR_UNSUPPORTED, "sequence too long for one launch");
+  if (!(scale > 0.f) || std::isinf(scale))
+    return fail(MI_ERR_INVALID_ARGUMENT, "scale must be a positive finite number");
+  if (!(softcap >= 0.f) || std::isinf(softcap))
+    return fail(MI_ERR_INVALID_ARGUMENT, "softcap must be finite and positive, or 0 for none");
+  return MI_OK;
+}
+
+// Unit dim stride and rows of whole aligned 16-byte chunks, 256 rows within the
+// 31-bit offsets of the tile loads.
+mi_status check_rows16(int dtype, std::initializer_list<std::pair<const void*, const int64_t*>> ts) {
+  for (const auto& t : ts) {
+    if (const mi_status st = check_attn_tensor("tensor", t.first, t.second); st != MI_OK) return st;
+    if (!aligned16(t.first, t.second, elem_size(dtype)))
+      return fail(MI_ERR_UNSUPPORTED, "rows must be 16-byte aligned, less than 8 MB apart");
+  }
+  return MI_OK;
+}
+
+mi_status check_mods(const mi_score_mods* m, const int32_t* tiles) {
+  if (m == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "mods: null pointer");
+  if (m->prefix_lens && !m->causal)
+    return fail(MI_ERR_INVALID_ARGUMENT, "prefix_lens: with causal only");
+  if (m->document_ids && (tiles == nullptr || ((uintptr_t)tiles) % 16))
+    return fail(MI_ERR_INVALID_ARGUMENT, "tiles: 16-byte aligned memory wanted");
+  return MI_OK;
+}
+
+mi::ScoreConst score_const(float scale, float softcap) {
+  mi::ScoreConst c = {};
+  c.c = scale * 1.4426950408889634f;
+  if (softcap > 0.f) {
+    c.kz = scale / softcap;
+    c.k1 = (float)(2.0 * 1.4426950408889634 * scale / softcap);
+    c.capl2 = (float)(1.4426950408889634 * softcap);
+  }
+  return c;
+}
+
+mi::SAttnArgs sattn_args(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                         const mi_score_mods& m, const int32_t* tiles) {
+  mi::SAttnArgs a = {};
+  a.slopes = m.slopes;
+  a.docs = m.document_ids;
+  a.prefix = m.prefix_lens;
+  a.ktiles = (const mi::DocTile*)tiles;
+  a.qtiles = a.ktiles + (int64_t)B * ((Sk + 63) / 64);
+  a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.Sq = Sq; a.Sk = Sk; a.D = D;
+  a.off = Sk - Sq;
+  a.dch = D * elem_size(dtype) / 16;
+  a.causal = m.causal ? 1 : 0;
+  a.scale = scale;
+  a.sc = score_const(scale, m.softcap);
+  return a;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t mi_sattn_tiles(int B, int Sq, int Sk) {
+  if (B <= 0 || Sq <= 0 || Sk <= 0) return 0;
+  return 4 * (int64_t)B * (((int64_t)Sq + 63) / 64 + ((int64_t)Sk + 63) / 64);
+}
+
+mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                       const mi_score_mods* mods, const void* q, const int64_t q_strides[4],
+                       const void* k, const int64_t k_strides[4], const void* v,
+                       const int64_t v_strides[4], void* o, const int64_t o_strides[4], float* lse,
+                       int32_t* tiles, void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_mods(mods, tiles)) != MI_OK) return st;
+  if ((st = check_sattn(dtype, B, H, Hk, Sq, Sk, D, scale, mods->softcap)) != MI_OK) return st;
+  if ((st = check_rows16(dtype, {{q, q_strides}, {k, k_strides}, {v, v_strides},
+                                 {o, o_strides}})) != MI_OK)
+    return st;
+  if (lse == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "lse: null pointer");
+  mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, scale, *mods, tiles);
+  a.q = targ(q, q_strides);
+  a.k = targ(k, k_strides);
+  a.v = targ(v, v_strides);
+  a.o = targ(o, o_strides);
+  a.lse = lse;
+  if (a.docs) {
+    st = launched(mi::launch_doc_tiles(a.docs, tiles, B, Sq, Sk, (hipStream_t)stream), "doc_tiles");
+    if (st != MI_OK) return st;
+  }
+  return launched(mi::launch_sattn_fwd(dtype, a, mods->softcap > 0.f, (hipStream_t)stream),
+                  "sattn_fwd");
+}
+
+int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
+  if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
+  return 2 * (int64_t)B * H * Sq;
+}
+
+mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                       const mi_score_mods* mods, const void* q, const int64_t q_strides[4],
+                       const void* k, const int64_t k_strides[4], const void* v,
+                       const int64_t v_strides[4], const void* o, const int64_t o_strides[4],
+                       const void* dout, const int64_t dout_strides[4], const float* lse,
+                       const int32_t* tiles, float* workspace, int64_t workspace_elems, void* dq,
+                       const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4],
+                       void* dv, const int64_t dv_strides[4], void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_mods(mods, tiles)) != MI_OK) return st;
+  if ((st = check_sattn(dtype, B, H, Hk, Sq, Sk, D, scale, mods->softcap)) != MI_OK) return st;
+  if ((st = check_rows16(dtype, {{q, q_strides}, {k, k_strides}, {v, v_strides}, {o, o_strides},
+                                 {dout, dout_strides}, {dq, dq_strides}, {dk, dk_strides},
+                                 {dv, dv_strides}})) != MI_OK)
+    return st;
+  if (lse == nullptr || workspace == nullptr || ((uintptr_t)workspace) % 16)
+    return fail(MI_ERR_INVALID_ARGUMENT, "lse / workspace: 16-byte aligned memory wanted");
+  const int64_t want = mi_sattn_bwd_workspace(dtype, B, H, Hk, Sq, Sk, D);
+  if (workspace_elems < want)
+    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted",
+                (long long)workspace_elems, (long long)want);
+  // delta and lse * log2(e), as for the attention without modified scores
+  mi::AttnArgs pre = {};
+  pre.o = targ(o, o_strides);
+  pre.dout = targ(dout, dout_strides);
+  pre.lse = const_cast<float*>(lse);
+  pre.delta = workspace;
+  pre.B = B; pre.H = H; pre.S = Sq; pre.D = D;
+  st = launched(mi::launch_attn_delta(dtype, pre, (hipStream_t)stream), "attn_delta");
+  if (st != MI_OK) return st;
+  mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, scale, *mods, tiles);
+  a.q = targ(q, q_strides);
+  a.k = targ(k, k_strides);
+  a.v = targ(v, v_strides);
+  a.dout = targ(dout, dout_strides);
+  a.dq = targ(dq, dq_strides);
+  a.dk = targ(dk, dk_strides);
+  a.dv = targ(dv, dv_strides);
+  a.delta = workspace;
+  a.lse2 = workspace + (int64_t)B * H * Sq;
+  return launched(mi::launch_sattn_bwd(dtype, a, mods->softcap > 0.f, (hipStream_t)stream),
+                  "sattn_bwd");
+}
+
+int64_t mi_decode_workspace(mi_dtype dtype, int B, int H, int Hk, int S, int D) {
+  if (check_sattn(dtype, B, H, Hk, 1, S, D, 1.f, 0.f) != MI_OK) return 0;
+  const int64_t n = mi::decode_splits(dtype, B, H, Hk, S, D);
+  return n == 1 ? 0 : (int64_t)B * H * n * (D + 2);
+}
+
+mi_status mi_decode_attn(mi_dtype dtype, int B, int H, int Hk, int S, int D, float scale,
+                         float softcap, const float* slopes, const int32_t* lengths,
+                         const void* q, const int64_t q_strides[3], const void* k,
+                         const int64_t k_strides[4], const void* v, const int64_t v_strides[4],
+                         void* o, const int64_t o_strides[3], float* workspace,
+                         int64_t workspace_elems, void* stream) {
+  MI_SOLE_COPY();
+  mi_status st;
+  if ((st = check_sattn(dtype, B, H, Hk, 1, S, D, scale, softcap)) != MI_OK) return st;
+  if ((st = check_rows16(dtype, {{k, k_strides}, {v, v_strides}})) != MI_OK) return st;
+  if ((st = check_pointers({q, o, q_strides, o_strides})) != MI_OK) return st;
+  const int esz = elem_size(dtype);
+  if (q_strides[2] != 1 || o_strides[2] != 1)
+    return fail(MI_ERR_INVALID_ARGUMENT, "dim stride must be 1");
+  if (((uintptr_t)q) % 16 || q_strides[0] * esz % 16 || q_strides[1] * esz % 16)
+    return fail(MI_ERR_UNSUPPORTED, "rows must be 16-byte aligned");
+  const int64_t want = mi_decode_workspace(dtype, B, H, Hk, S, D);
+  if (want && (workspace == nullptr || workspace_elems < want))
+    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted",
+                (long long)workspace_elems, (long long)want);
+  mi::DecodeArgs a = {};
+  a.q = q;
+  a.q_sb = q_strides[0]; a.q_sh = q_strides[1];
+  a.o = o;
+  a.o_sb = o_strides[0]; a.o_sh = o_strides[1];
+  a.k = targ(k, k_strides);
+  a.v = targ(v, v_strides);
+  a.slopes = slopes;
+  a.lengths = lengths;
+  a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.S = S; a.D = D;
+  a.dch = D * esz / 16;
+  a.splits = mi::decode_splits(dtype, B, H, Hk, S, D);
+  a.sc = score_const(scale, softcap);
+  a.part = workspace;
+  a.ml = workspace + (int64_t)B * H * a.splits * D;
+  return launched(mi::launch_decode(dtype, a, softcap > 0.f, (hipStream_t)stream), "decode");
+}
+
+}  // extern "C"

@@ -163,6 +163,45 @@ int wgrad_splits(int64_t M, int64_t N, int64_t K);
 bool wgrad_suits(int64_t M, int64_t N, int64_t K);
 hipError_t launch_wgrad(int dtype, WgradArgs a, hipStream_t st);
 
+// Rotary embedding of q and k at given positions, alone or behind the norm of
+// each head (rotary.hip).
+struct RotaryTensor {
+  const void* x;   // [S, B, heads, D] by element strides (the forward's input)
+  const void* dy;  // mode 2: gradient of the output
+  void* out;       // output; mode 2: dx
+  int64_t x_ss, x_sb, x_sh, x_sd, dy_ss, dy_sb, dy_sh, dy_sd, o_ss, o_sb, o_sh, o_sd;
+  const void* w;   // modes 1, 2: [D]
+  void* dw;        // mode 2
+  int heads;
+};
+struct RotaryArgs {
+  RotaryTensor t[2];  // q, k
+  const void *cos, *sin;
+  int64_t cs_s, cs_i, ss_s, ss_i;  // table strides (position, pair)
+  int64_t T;                       // table rows
+  const void* pos;                 // positions by token, or null: the row index
+  int64_t pos_ss, pos_sb;
+  int pos64, tab_dt, w_dt;
+  int S, B, D, R, interleaved, inverse;
+  float eps;
+  float* part;    // mode 2: [blocks[0] + blocks[1], D]
+  int blocks[2];
+};
+int rotary_grad_blocks(int64_t rows);
+bool rotary_vec_ok(int dtype, int D, int R);
+// mode 0: rotation alone, 1: norm and rotation, 2: backward of 1.  vec: whole
+// 16-byte chunks of everything, aligned.
+hipError_t launch_rotary(int dtype, int mode, const RotaryArgs& a, bool vec, hipStream_t st);
+
+// Attention with modified scores (sattn_device.h has the argument blocks).
+struct SAttnArgs;
+struct DecodeArgs;
+hipError_t launch_doc_tiles(const int* docs, void* tiles, int B, int Sq, int Sk, hipStream_t st);
+hipError_t launch_sattn_fwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st);
+hipError_t launch_sattn_bwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st);
+int decode_splits(int dtype, int B, int H, int Hk, int S, int D);
+hipError_t launch_decode(int dtype, const DecodeArgs& a, bool cap, hipStream_t st);
+
 // The optimizer step (model_ops.hip).  Squared gradient norm into out[0] via
 // adam_parts() partial sums; the AdamW step over the flat buffers with
 // hp = {1 - lr*wd, 1 - beta1, beta2, 1 - beta2, lr / (1 - beta1^t),

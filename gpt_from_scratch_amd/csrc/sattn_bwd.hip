@@ -1,0 +1,475 @@
+// sattn_bwd.hip — backward of attention with modified scores, for bf16, f16 and
+// fp32 (sattn_device.h has the forward's mathematics).  With lse and
+// delta = rowsum(dO * O) from before (attn_delta):
+//   P = exp(x - lse);  dV = P^T dO;  dP = dO V^T;  dx = P * (dP - delta)
+//   dz = dx * (1 - tanh^2(z / cap));  dQ = scale * dz K;  dK = scale * dz^T Q
+// dK and dV of a key head sum over the query heads that share it.
+//
+// Two kinds of workgroup, as in attn_bwd.hip, both without atomics, so results
+// repeat bit for bit:
+//   dK/dV: 128 keys of one key head, looping over the group's query heads and
+//     their query tiles; S = Q K^T and dP = dO V^T keep a key per lane, so P and
+//     dz feed dV^T = dO^T P and dK^T = Q^T dz from the accumulators.  The dP
+//     accumulators start at +delta and V is negated, so they end at delta - dP;
+//   dQ: 128 queries of one head, looping over key tiles; a query per lane.
+// Five products in dK/dV and dQ together recompute S and dP once each more than
+// the least: 7 products against 5, in exchange for no atomics on dQ.
+// Tiles without a visible pair are not visited, as in the forward (TileScan).
+#include <type_traits>
+
+#include "sattn_device.h"
+
+namespace mi {
+
+namespace {
+
+// Rows of a streamed tile: two tiles of two tensors, twice buffered.
+template <typename E, int D>
+constexpr int kTile = Lay<E, D>::RB > 128 ? 32 : 64;
+
+template <typename E, int D>
+constexpr int kWavesPerSimd = Lay<E, D>::RB > 256 ? 1 : 2;
+
+__device__ __forceinline__ const char* head_bytes(const TensorArg& t, int b, int h, int esz) {
+  return (const char*)t.ptr + (b * t.sb + h * t.sh) * esz;
+}
+
+// A wave's own 32 rows as B operands: lane: row l32, chunk 2 ks + g.
+template <typename E, int D>
+__device__ __forceinline__ void load_own(const TensorArg& t, int b, int h, int row, bool valid,
+                                         int dch, int g, u32x4 (&x)[Lay<E, D>::KS]) {
+  using L = Lay<E, D>;
+  const char* p = head_bytes(t, b, h, L::ESZ) + row * t.ss * L::ESZ;
+#pragma unroll
+  for (int ks = 0; ks < L::KS; ++ks)
+    x[ks] = valid && 2 * ks + g < dch ? *(const u32x4*)(p + 16 * (2 * ks + g)) : u32x4{0, 0, 0, 0};
+}
+
+// P and the factor of dx that the cap's derivative brings.
+template <typename E, bool CAP, bool BIAS>
+__device__ __forceinline__ float prob(float s, float dist, float slope2, float lse2,
+                                      const ScoreConst& k, float& deriv) {
+  if constexpr (!CAP && !BIAS) {
+    return fast_exp2(__builtin_fmaf(s, k.c, -lse2));
+  } else {
+    float t;
+    const float x = score<E, CAP, BIAS>(s, dist, slope2, k, t);
+    if constexpr (CAP) deriv = __builtin_fmaf(-t, t, 1.f);
+    return fast_exp2(x - lse2);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// dK, dV
+// ---------------------------------------------------------------------------
+template <typename E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(SAttnArgs a) {
+  using L = Lay<E, D>;
+  constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
+  constexpr bool K_IN_LDS = L::RB > 128;  // K and V rows and both sums pass 256 registers
+  __shared__ __attribute__((aligned(16))) char Q0[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char Q1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char G0[T * L::RB];  // dO
+  __shared__ __attribute__((aligned(16))) char G1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) float S0[3 * T];  // lse2, delta, document ids
+  __shared__ __attribute__((aligned(16))) float S1[3 * T];
+  __shared__ __attribute__((aligned(16))) char KL[K_IN_LDS ? OWN * L::RB : 16];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Sq = a.Sq, Sk = a.Sk;
+  const int BHk = a.B * a.Hk;
+  // key tile 0 sees the most queries under a causal mask: first
+  const int kt = blockIdx.x / BHk, bk = blockIdx.x % BHk, b = bk / a.Hk, hk = bk % a.Hk;
+  const int k0 = kt * OWN, kw = k0 + 32 * wave, krow = kw + l32;
+  const bool wave_valid = kw < Sk;
+  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const int kdoc = docs && krow < Sk ? docs[krow] : 0;
+  // first query position that sees this lane's key, and the wave's first
+  int qfirst = 0, wfirst = 0;
+  if (a.causal) {
+    qfirst = krow < prefix ? 0 : krow;
+    wfirst = kw < prefix ? 0 : kw;
+  }
+  if (kdoc < 0) qfirst = 0x7fffffff;
+
+  char* const kl = KL + (K_IN_LDS ? wave * 32 * L::RB : 0);
+  u32x4 kf[L::KS], vn[L::KS];
+  load_own<E, D>(a.k, b, hk, krow, krow < Sk, a.dch, g, kf);
+  load_own<E, D>(a.v, b, hk, krow, krow < Sk, a.dch, g, vn);
+  constexpr uint32_t neg = L::ESZ == 2 ? 0x80008000u : 0x80000000u;
+#pragma unroll
+  for (int ks = 0; ks < L::KS; ++ks) vn[ks] ^= neg;
+  Reads<E, D> rd;
+  rd.init(lane);
+  if constexpr (K_IN_LDS) {
+#pragma unroll
+    for (int ks = 0; ks < L::KS; ++ks)
+      *(u32x4*)(kl + 256 * (ks / rd.NR) + rd.r[ks % rd.NR]) = kf[ks];
+  }
+
+  const int kmax = min(k0 + OWN, Sk) - 1;
+  DocRange own = {0, 0, false};
+  if (docs) own = doc_range(docs, k0, kmax - k0 + 1, lane);
+  const DocTile* qtiles = a.qtiles + (int64_t)b * ((Sq + 63) / 64);
+  auto look = [&](int t) __attribute__((always_inline)) {
+    const int q0 = t * T, p0 = a.off + q0, p1 = a.off + min(q0 + T, Sq) - 1;
+    bool live = !a.causal || p1 >= k0 || k0 < prefix;
+    bool full = q0 + T <= Sq && (!a.causal || p0 >= kmax || kmax < prefix);
+    bool pad = false;
+    if (docs) {
+      const DocTile w = qtiles[q0 >> 6];
+      live = live && w.lo <= own.hi && w.hi >= own.lo;
+      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
+      pad = w.pad;
+    }
+    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+  };
+  const int nqt = (Sq + T - 1) / T;
+  // the group's query heads one after another
+  int h = hk * a.G;
+  const int hend = h + a.G;
+  TileScan scan;
+  scan.n = nqt;
+  auto next = [&](int& head) __attribute__((always_inline)) {
+    int t = scan.next(lane, look);
+    while (t < 0 && head + 1 < hend) {
+      ++head;
+      scan = TileScan();
+      scan.n = nqt;
+      t = scan.next(lane, look);
+      if (t < 0) head = hend - 1;  // no tile for one head: none for any
+    }
+    return t;
+  };
+
+  Stage<E, D, T> qsrc, gsrc;
+  qsrc.init(a.q, b, 0, a.dch, lane, wave);
+  gsrc.init(a.dout, b, 0, a.dch, lane, wave);
+  const char *qbase = qsrc.base, *gbase = gsrc.base;
+  auto fetch = [&](int t, int head, char* qb, char* gb, float* sb) __attribute__((always_inline)) {
+    const int q0 = (t & kTileIndex) * T;
+    qsrc.base = qbase + head * a.q.sh * L::ESZ;
+    gsrc.base = gbase + head * a.dout.sh * L::ESZ;
+    if (t & kPad) {
+      qsrc.load_padded(q0, Sq, qb, lane, wave, docs + a.off + q0);
+      gsrc.load_padded(q0, Sq, gb, lane, wave, docs + a.off + q0);
+    } else {
+      qsrc.load(q0, Sq, qb, wave);
+      gsrc.load(q0, Sq, gb, wave);
+    }
+    const int nr = 4 * min(T, Sq - q0);
+    const int64_t row = ((int64_t)b * a.H + head) * Sq + q0;
+    if (lane < T) {
+      if (wave == 0) buffer_load_lds4(tile_rsrc(a.lse2 + row, nr), 4 * lane, sb);
+      if (wave == 1) buffer_load_lds4(tile_rsrc(a.delta + row, nr), 4 * lane, sb + T);
+      if (wave == 2 && docs)
+        buffer_load_lds4(tile_rsrc(docs + a.off + q0, nr), 4 * lane, sb + 2 * T);
+    }
+  };
+
+  f32x16 dk[L::DB], dv[L::DB];
+#pragma unroll
+  for (int i = 0; i < L::DB; ++i) dk[i] = dv[i] = f32x16{};
+
+  int cur = next(h);
+  float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+  if (cur >= 0) fetch(cur, h, Q0, G0, S0);
+  __syncthreads();
+  auto step = [&](int cur, int nxt, int hnext, auto slot) __attribute__((always_inline)) {
+    constexpr int I = decltype(slot)::value;
+    const char* qt = I ? Q1 : Q0;
+    const char* gt = I ? G1 : G0;
+    const float* st = I ? S1 : S0;
+    if (nxt >= 0) fetch(nxt, hnext, I ? Q0 : Q1, I ? G0 : G1, I ? S0 : S1);
+    rd.refresh();
+    const int q0 = (cur & kTileIndex) * T, p0 = a.off + q0;
+    if (wave_valid && p0 + T - 1 >= wfirst) {
+      const bool full = cur & kFull;
+      u32x4 pb[TB][L::NG], sb[TB][L::NG];
+#pragma unroll
+      for (int qb = 0; qb < TB; ++qb) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          const f32x4 d4 = *(const f32x4*)(st + T + 32 * qb + 8 * jj + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) dp[4 * jj + i] = d4[i];
+        }
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks)
+          s = Elem<E>::mfma(rd.row(qt, qb, ks), K_IN_LDS ? rd.row(kl, 0, ks) : kf[ks],
+                            ks == 0 ? f32x16{} : s);
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks)
+          dp = Elem<E>::mfma(rd.row(gt, qb, ks), vn[ks], dp);
+        // query of register r: q0 + 32 qb + 8 (r / 4) + 4 g + r % 4
+        const float d0 = (float)(p0 - krow + 32 * qb + 4 * g);
+#pragma unroll
+        for (int jj = 0; jj < 4; ++jj) {
+          const f32x4 l4 = *(const f32x4*)(st + 32 * qb + 8 * jj + 4 * g);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = 4 * jj + i;
+            float deriv = 1.f;
+            const float p =
+                prob<E, CAP, BIAS>(s[r], d0 + (8 * jj + i), slope2, l4[i], a.sc, deriv);
+            s[r] = p;
+            dp[r] = -(p * dp[r]);
+            if constexpr (CAP) dp[r] *= deriv;
+          }
+        }
+        if (!full) {
+          const int base = q0 + 32 * qb + 4 * g;
+          const int lo = qfirst == 0x7fffffff ? qfirst : qfirst - a.off - base, hi = Sq - base;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            const int n = 8 * (r >> 2) + (r & 3);
+            if (n < lo || n >= hi) s[r] = dp[r] = 0.f;
+          }
+          if (docs) {
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const i32x4 d4 = *(const i32x4*)(st + 2 * T + 32 * qb + 8 * jj + 4 * g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (d4[i] != kdoc) s[4 * jj + i] = dp[4 * jj + i] = 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng) {
+          pb[qb][ng] = Elem<E>::operand(s, ng);
+          sb[qb][ng] = Elem<E>::operand(dp, ng);
+        }
+      }
+#pragma unroll
+      for (int qb = 0; qb < TB; ++qb)
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng)
+#pragma unroll
+          for (int db = 0; db < L::DB; ++db) {
+            dv[db] = Elem<E>::mfma(rd.col(gt, qb, ng, db), pb[qb][ng], dv[db]);
+            dk[db] = Elem<E>::mfma(rd.col(qt, qb, ng, db), sb[qb][ng], dk[db]);
+          }
+    }
+    __syncthreads();
+  };
+  while (cur >= 0) {
+    int nxt = next(h);
+    step(cur, nxt, h, std::integral_constant<int, 0>{});
+    if (BIAS) slope2 = a.slopes[h] * kLog2e;
+    if ((cur = nxt) < 0) break;
+    nxt = next(h);
+    step(cur, nxt, h, std::integral_constant<int, 1>{});
+    if (BIAS) slope2 = a.slopes[h] * kLog2e;
+    cur = nxt;
+  }
+
+  if (!wave_valid) return;
+  // idle now: the wave's K rows, or one of the tile buffers
+  char* stage = K_IN_LDS ? kl : wave == 0 ? Q0 : wave == 1 ? Q1 : wave == 2 ? G0 : G1;
+  const int nrows = min(32, Sk - kw);
+  store_rows<E, D>(dv, 1.f, stage,
+                   (char*)a.dv.ptr + (b * a.dv.sb + hk * a.dv.sh + kw * a.dv.ss) * L::ESZ,
+                   a.dv.ss * L::ESZ, a.dch, nrows);
+  store_rows<E, D>(dk, a.scale, stage,
+                   (char*)a.dk.ptr + (b * a.dk.sb + hk * a.dk.sh + kw * a.dk.ss) * L::ESZ,
+                   a.dk.ss * L::ESZ, a.dch, nrows);
+}
+
+// ---------------------------------------------------------------------------
+// dQ
+// ---------------------------------------------------------------------------
+template <typename E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SAttnArgs a) {
+  using L = Lay<E, D>;
+  constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
+  __shared__ __attribute__((aligned(16))) char K0[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char K1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char V0[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char V1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) int I0[T];
+  __shared__ __attribute__((aligned(16))) int I1[T];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Sq = a.Sq, Sk = a.Sk;
+  const int BH = a.B * a.H, BHk = a.B * a.Hk;
+  const int nqt = (Sq + OWN - 1) / OWN;
+  const int qt = nqt - 1 - blockIdx.x / BH;
+  const int n = blockIdx.x % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
+  const int h = hk * a.G + n / BHk;
+  const int q0 = qt * OWN, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
+  const bool wave_valid = qw < Sq;
+  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+  const int qdoc = docs && qrow < Sq ? docs[qpos] : 0;
+  int klast = Sk - 1, wlast = Sk - 1;
+  if (a.causal) {
+    klast = min(max(qpos, prefix - 1), Sk - 1);
+    wlast = max(a.off + min(qw + 31, Sq - 1), prefix - 1);
+  }
+  if (qdoc < 0) klast = -1;
+
+  u32x4 qf[L::KS], df[L::KS];
+  load_own<E, D>(a.q, b, h, qrow, qrow < Sq, a.dch, g, qf);
+  load_own<E, D>(a.dout, b, h, qrow, qrow < Sq, a.dch, g, df);
+  const int64_t row = ((int64_t)b * a.H + h) * Sq + qrow;
+  const float lse2 = qrow < Sq ? a.lse2[row] : 0.f;
+  const float ndelta = qrow < Sq ? -a.delta[row] : 0.f;
+
+  const int pmin = a.off + q0, pmax = a.off + min(q0 + OWN, Sq) - 1;
+  DocRange own = {0, 0, false};
+  if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
+  const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + 63) / 64);
+  TileScan scan;
+  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk;
+  scan.n = (kend + T - 1) / T;
+  auto look = [&](int t) __attribute__((always_inline)) {
+    const int k0 = t * T;
+    bool live = !a.causal || k0 <= pmax || k0 < prefix;
+    bool full = k0 + T <= Sk && (!a.causal || k0 + T - 1 <= pmin || k0 + T <= prefix);
+    bool pad = false;
+    if (docs) {
+      const DocTile w = ktiles[k0 >> 6];
+      live = live && w.lo <= own.hi && w.hi >= own.lo;
+      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
+      pad = w.pad;
+    }
+    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+  };
+
+  Stage<E, D, T> ksrc, vsrc;
+  ksrc.init(a.k, b, hk, a.dch, lane, wave);
+  vsrc.init(a.v, b, hk, a.dch, lane, wave);
+  Reads<E, D> rd;
+  rd.init(lane);
+  auto fetch = [&](int t, char* kb, char* vb, int* ib) __attribute__((always_inline)) {
+    const int k0 = (t & kTileIndex) * T;
+    if (t & kPad) {
+      ksrc.load_padded(k0, Sk, kb, lane, wave, docs + k0);
+      vsrc.load_padded(k0, Sk, vb, lane, wave, docs + k0);
+    } else {
+      ksrc.load(k0, Sk, kb, wave);
+      vsrc.load(k0, Sk, vb, wave);
+    }
+    if (docs && wave == 0 && lane < T)
+      buffer_load_lds4(tile_rsrc(docs + k0, 4 * min(T, Sk - k0)), 4 * lane, (float*)ib);
+  };
+
+  f32x16 acc[L::DB];
+#pragma unroll
+  for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  int cur = scan.next(lane, look);
+  if (cur >= 0) {
+    fetch(cur, K0, V0, I0);
+    __syncthreads();
+  }
+  auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
+    constexpr int I = decltype(slot)::value;
+    const char* kt = I ? K1 : K0;
+    const char* vt = I ? V1 : V0;
+    const int* it = I ? I1 : I0;
+    if (nxt >= 0) fetch(nxt, I ? K0 : K1, I ? V0 : V1, I ? I0 : I1);
+    rd.refresh();
+    const int k0 = (cur & kTileIndex) * T;
+    if (wave_valid && k0 <= wlast) {
+      u32x4 sb[TB][L::NG];
+#pragma unroll
+      for (int kb = 0; kb < TB; ++kb) {
+        f32x16 s, dp;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = ndelta;
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks)
+          s = Elem<E>::mfma(rd.row(kt, kb, ks), qf[ks], ks == 0 ? f32x16{} : s);
+#pragma unroll
+        for (int ks = 0; ks < L::KS; ++ks) dp = Elem<E>::mfma(rd.row(vt, kb, ks), df[ks], dp);
+        const float d0 = (float)(qpos - k0 - 32 * kb - 4 * g);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float deriv = 1.f;
+          const float p = prob<E, CAP, BIAS>(s[r], d0 - (8 * (r >> 2) + (r & 3)), slope2, lse2, a.sc,
+                                             deriv);
+          dp[r] *= p;
+          if constexpr (CAP) dp[r] *= deriv;
+        }
+        if (!(cur & kFull)) {
+          const int rel = klast - k0 - 32 * kb - 4 * g;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (8 * (r >> 2) + (r & 3) > rel) dp[r] = 0.f;
+          if (docs) {
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const i32x4 d4 = *(const i32x4*)(it + 32 * kb + 8 * jj + 4 * g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (d4[i] != qdoc) dp[4 * jj + i] = 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng) sb[kb][ng] = Elem<E>::operand(dp, ng);
+      }
+#pragma unroll
+      for (int kb = 0; kb < TB; ++kb)
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng)
+#pragma unroll
+          for (int db = 0; db < L::DB; ++db)
+            acc[db] = Elem<E>::mfma(rd.col(kt, kb, ng, db), sb[kb][ng], acc[db]);
+    }
+    __syncthreads();
+  };
+  while (cur >= 0) {
+    int nxt = scan.next(lane, look);
+    step(cur, nxt, std::integral_constant<int, 0>{});
+    if ((cur = nxt) < 0) break;
+    nxt = scan.next(lane, look);
+    step(cur, nxt, std::integral_constant<int, 1>{});
+    cur = nxt;
+  }
+
+  if (!wave_valid) return;
+  char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
+  store_rows<E, D>(acc, a.scale, stage,
+                   (char*)a.dq.ptr + (b * a.dq.sb + h * a.dq.sh + qw * a.dq.ss) * L::ESZ,
+                   a.dq.ss * L::ESZ, a.dch, min(32, Sq - qw));
+}
+
+template <typename E, int D, bool CAP, bool BIAS>
+hipError_t launch_cb(const SAttnArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((sattn_dkdv_kernel<E, D, CAP, BIAS>), dim3((a.Sk + 127) / 128 * a.B * a.Hk),
+                     dim3(256), 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((sattn_dq_kernel<E, D, CAP, BIAS>), dim3((a.Sq + 127) / 128 * a.B * a.H),
+                     dim3(256), 0, st, a);
+  return hipGetLastError();
+}
+
+template <typename E, int D>
+hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
+  if (cap && a.slopes) return launch_cb<E, D, true, true>(a, st);
+  if (cap) return launch_cb<E, D, true, false>(a, st);
+  if (a.slopes) return launch_cb<E, D, false, true>(a, st);
+  return launch_cb<E, D, false, false>(a, st);
+}
+
+template <typename E>
+hipError_t launch_e(const SAttnArgs& a, bool cap, hipStream_t st) {
+  return a.D <= 64 ? launch_d<E, 64>(a, cap, st) : launch_d<E, 128>(a, cap, st);
+}
+
+}  // namespace
+
+hipError_t launch_sattn_bwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st) {
+  if (dtype == 0) return launch_e<F32>(a, cap, st);
+  return dtype == 1 ? launch_e<F16>(a, cap, st) : launch_e<BF16>(a, cap, st);
+}
+
+}  // namespace mi

@@ -1,0 +1,280 @@
+// sattn_fwd.hip — forward of attention with modified scores (capped, biased by
+// distance, masked by documents or a prefix, key heads shared by query heads),
+// for bf16, f16 and fp32.  The mathematics is at the top of sattn_device.h.
+//
+// Bound by the matrix cores for plain scores; a cap adds two transcendentals per
+// score to the softmax's one, which take longer than the score's products.
+//
+// Work decomposition, as in attn_fwd.hip: a workgroup (4 waves) owns 128 query
+// rows of one head, wave w rows [32w, 32w + 32); S^T = K Q^T and O^T = V^T P^T
+// keep a query per lane, so the softmax's statistics are per-lane scalars and P
+// feeds the second product from the accumulators; 64-key tiles of K and V come
+// in by direct global -> LDS loads, double buffered, one barrier per tile.
+//   * Which key tiles a workgroup visits is found 64 at a time by ballot
+//     (TileScan) from positions, the prefix and the 64-key ranges of document
+//     ids: tiles without a visible pair cost nothing, tiles where every pair is
+//     visible run without mask code.
+//   * Query heads that share a key head go to the same XCD (workgroups are dealt
+//     round robin over the 8 XCDs), so that its L2 reads K and V once for all.
+//   * Head dims below 64 and between 64 and 128 run in the next layout with zero
+//     chunks.
+#include <type_traits>
+
+#include "sattn_device.h"
+
+namespace mi {
+
+namespace {
+
+// Document id ranges of each 64 keys and each 64 queries: a wave per record.
+__global__ __launch_bounds__(256) void doc_tiles_kernel(const int* docs, DocTile* out, int B, int Sq,
+                                                        int Sk, int nk, int nq) {
+  const int lane = threadIdx.x & 63;
+  const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (i >= (int64_t)B * (nk + nq)) return;
+  const bool key = i < (int64_t)B * nk;
+  const int64_t j = key ? i : i - (int64_t)B * nk;
+  const int per = key ? nk : nq, b = (int)(j / per), t = (int)(j % per);
+  const int off = key ? 0 : Sk - Sq, rows = key ? Sk : Sq;
+  const DocRange r = doc_range(docs + (int64_t)b * Sk, off + 64 * t, min(64, rows - 64 * t), lane);
+  if (lane == 0) out[i] = DocTile{r.lo, r.hi, r.pad, 0};
+}
+
+constexpr float kSlack = 8.f;  // log2 units a score may exceed the running reference by
+
+template <typename E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_kernel(SAttnArgs a) {
+  using L = Lay<E, D>;
+  constexpr int BQ = 128, BK = 64;
+  __shared__ __attribute__((aligned(16))) char K0[BK * L::RB];
+  __shared__ __attribute__((aligned(16))) char K1[BK * L::RB];
+  __shared__ __attribute__((aligned(16))) char V0[BK * L::RB];
+  __shared__ __attribute__((aligned(16))) char V1[BK * L::RB];
+  __shared__ __attribute__((aligned(16))) int I0[BK];  // document ids of the keys
+  __shared__ __attribute__((aligned(16))) int I1[BK];
+
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int Sq = a.Sq, Sk = a.Sk;
+
+  // last query tiles first (the longest under a causal mask); within a tile, key
+  // heads run fastest, then the query heads of a group
+  const int BH = a.B * a.H, BHk = a.B * a.Hk;
+  const int nqt = (Sq + BQ - 1) / BQ;
+  const int qt = nqt - 1 - blockIdx.x / BH;
+  const int n = blockIdx.x % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
+  const int h = hk * a.G + n / BHk;
+
+  const int q0 = qt * BQ, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
+  const bool wave_valid = qw < Sq;
+  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
+
+  const char* qp = (const char*)a.q.ptr + (b * a.q.sb + h * a.q.sh + qrow * a.q.ss) * L::ESZ;
+  u32x4 qf[L::KS];
+#pragma unroll
+  for (int ks = 0; ks < L::KS; ++ks)
+    qf[ks] = qrow < Sq && 2 * ks + g < a.dch ? *(const u32x4*)(qp + 16 * (2 * ks + g))
+                                              : u32x4{0, 0, 0, 0};
+  const int qdoc = docs && qrow < Sq ? docs[qpos] : 0;
+  // last key that position and sequence end leave visible; none for padding
+  int klast = Sk - 1, wlast = Sk - 1;
+  if (a.causal) {
+    klast = min(max(qpos, prefix - 1), Sk - 1);
+    wlast = max(a.off + min(qw + 31, Sq - 1), prefix - 1);
+  }
+  if (qdoc < 0) klast = -1;
+
+  const int pmin = a.off + q0, pmax = a.off + min(q0 + BQ, Sq) - 1;
+  DocRange own = {0, 0, false};
+  if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
+  const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + BK - 1) / BK);
+  TileScan scan;
+  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk;
+  scan.n = (kend + BK - 1) / BK;
+  auto look = [&](int t) __attribute__((always_inline)) {
+    const int k0 = t * BK;
+    bool live = !a.causal || k0 <= pmax || k0 < prefix;
+    bool full = k0 + BK <= Sk && (!a.causal || k0 + BK - 1 <= pmin || k0 + BK <= prefix);
+    bool pad = false;
+    if (docs) {
+      const DocTile w = ktiles[t];
+      live = live && w.lo <= own.hi && w.hi >= own.lo;
+      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
+      pad = w.pad;
+    }
+    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+  };
+
+  Stage<E, D, BK> ksrc, vsrc;
+  ksrc.init(a.k, b, hk, a.dch, lane, wave);
+  vsrc.init(a.v, b, hk, a.dch, lane, wave);
+  Reads<E, D> rd;
+  rd.init(lane);
+
+  auto fetch = [&](int t, char* kb, char* vb, int* ib) __attribute__((always_inline)) {
+    const int k0 = (t & kTileIndex) * BK;
+    if (t & kPad) {
+      ksrc.load_padded(k0, Sk, kb, lane, wave, docs + k0);
+      vsrc.load_padded(k0, Sk, vb, lane, wave, docs + k0);
+    } else {
+      ksrc.load(k0, Sk, kb, wave);
+      vsrc.load(k0, Sk, vb, wave);
+    }
+    if (docs && wave == 0)
+      buffer_load_lds4(tile_rsrc(docs + k0, 4 * min(BK, Sk - k0)), 4 * lane, (float*)ib);
+  };
+
+  f32x16 acc[L::DB];
+#pragma unroll
+  for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  float m_run = -INFINITY, l_run = 0.f;
+  // factor that takes a score to log2 units
+  const float c = CAP || BIAS ? 1.f : a.sc.c;
+
+  int cur = scan.next(lane, look);
+  if (cur >= 0) {
+    fetch(cur, K0, V0, I0);
+    __syncthreads();
+  }
+  auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
+    constexpr int I = decltype(slot)::value;
+    const char* kt = I ? K1 : K0;
+    const char* vt = I ? V1 : V0;
+    const int* it = I ? I1 : I0;
+    if (nxt >= 0) fetch(nxt, I ? K0 : K1, I ? V0 : V1, I ? I0 : I1);
+    rd.refresh();
+    const int k0 = (cur & kTileIndex) * BK;
+    if (wave_valid && k0 <= wlast) {
+      f32x16 s[2];
+#pragma unroll
+      for (int ks = 0; ks < L::KS; ++ks)
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+          s[kb] = Elem<E>::mfma(rd.row(kt, kb, ks), qf[ks], ks == 0 ? f32x16{} : s[kb]);
+      if constexpr (CAP || BIAS) {
+        const float d0 = (float)(qpos - k0 - 4 * g);
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) {
+            float t;
+            s[kb][r] = score<E, CAP, BIAS>(s[kb][r], d0 - (32 * kb + 8 * (r >> 2) + (r & 3)), slope2,
+                                           a.sc, t);
+          }
+      }
+      if (!(cur & kFull)) {
+        const int rel = klast - k0 - 4 * g;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (32 * kb + 8 * (r >> 2) + (r & 3) > rel) s[kb][r] = -INFINITY;
+        if (docs) {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int jj = 0; jj < 4; ++jj) {
+              const i32x4 d4 = *(const i32x4*)(it + 32 * kb + 8 * jj + 4 * g);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (d4[i] != qdoc) s[kb][4 * jj + i] = -INFINITY;
+            }
+        }
+      }
+      float mx = vmax(s[0][0], s[0][1]);
+#pragma unroll
+      for (int i = 2; i < 32; i += 2) mx = vmax(vmax(mx, s[i >> 4][i & 15]), s[i >> 4][(i & 15) + 1]);
+      mx = max_halves(mx) * c;
+      // The reference moves only when a score passes it by more than kSlack:
+      // P stays below 2^8, and O and l share the reference whatever it is.
+      if (__any(mx > m_run + kSlack)) {
+        const float m_new = fmaxf(m_run, mx);
+        const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        l_run *= alpha;
+#pragma unroll
+        for (int db = 0; db < L::DB; ++db) acc[db] *= alpha;
+        m_run = m_new;
+      }
+      const float ref = m_run == -INFINITY ? 0.f : m_run;  // a row that has seen no key yet
+      u32x4 p[2][L::NG];
+      float ps[2] = {0.f, 0.f};
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][r] = fast_exp2(__builtin_fmaf(s[kb][r], c, -ref));
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng) {
+          p[kb][ng] = Elem<E>::operand(s[kb], ng);
+          // P as rounded for the product, so that O / l normalises what it applied
+          ps[ng & 1] = Elem<E>::sum(p[kb][ng], ps[ng & 1]);
+        }
+      }
+      l_run += ps[0] + ps[1];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng)
+#pragma unroll
+          for (int db = 0; db < L::DB; ++db)
+            acc[db] = Elem<E>::mfma(rd.col(vt, kb, ng, db), p[kb][ng], acc[db]);
+    }
+    __syncthreads();
+  };
+  while (cur >= 0) {
+    int nxt = scan.next(lane, look);
+    step(cur, nxt, std::integral_constant<int, 0>{});
+    if ((cur = nxt) < 0) break;
+    nxt = scan.next(lane, look);
+    step(cur, nxt, std::integral_constant<int, 1>{});
+    cur = nxt;
+  }
+
+  if (!wave_valid) return;
+  // a row without a visible key: O = 0, lse = -inf
+  const float l = sum_halves(l_run);
+  char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
+  store_rows<E, D>(acc, l == 0.f ? 0.f : 1.f / l, stage,
+                   (char*)a.o.ptr + (b * a.o.sb + h * a.o.sh + qw * a.o.ss) * L::ESZ,
+                   a.o.ss * L::ESZ, a.dch, min(32, Sq - qw));
+  if (g == 0 && qrow < Sq)
+    a.lse[((int64_t)b * a.H + h) * Sq + qrow] =
+        l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
+}
+
+template <typename E, int D>
+hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
+  const dim3 grid((a.Sq + 127) / 128 * a.B * a.H), block(256);
+  if (cap && a.slopes)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, true>), grid, block, 0, st, a);
+  else if (cap)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, false>), grid, block, 0, st, a);
+  else if (a.slopes)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, true>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, false>), grid, block, 0, st, a);
+  return hipGetLastError();
+}
+
+template <typename E>
+hipError_t launch_e(const SAttnArgs& a, bool cap, hipStream_t st) {
+  return a.D <= 64 ? launch_d<E, 64>(a, cap, st) : launch_d<E, 128>(a, cap, st);
+}
+
+}  // namespace
+
+hipError_t launch_doc_tiles(const int* docs, void* tiles, int B, int Sq, int Sk, hipStream_t st) {
+  const int nk = (Sk + 63) / 64, nq = (Sq + 63) / 64;
+  const int64_t n = (int64_t)B * (nk + nq);
+  hipLaunchKernelGGL(doc_tiles_kernel, dim3((uint32_t)((n + 3) / 4)), dim3(256), 0, st, docs,
+                     (DocTile*)tiles, B, Sq, Sk, nk, nq);
+  return hipGetLastError();
+}
+
+hipError_t launch_sattn_fwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st) {
+  if (dtype == 0) return launch_e<F32>(a, cap, st);
+  return dtype == 1 ? launch_e<F16>(a, cap, st) : launch_e<BF16>(a, cap, st);
+}
+
+}  // namespace mi

@@ -30,6 +30,8 @@
 #include <ATen/autocast_mode.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 
 #include <cstring>
@@ -48,7 +50,10 @@ using torch::autograd::variable_list;
   X(mi_rope) X(mi_rope_qk) X(mi_xent_fwd) X(mi_xent_bwd) X(mi_rmsnorm_fwd)                 \
   X(mi_rmsnorm_bwd_workspace) X(mi_rmsnorm_bwd) X(mi_rmsnorm_bwd_acc)                      \
   X(mi_rmsnorm_add_fwd) X(mi_rmsnorm_add_bwd) X(mi_rmsnorm_add_bwd_acc) X(mi_swiglu_fwd)   \
-  X(mi_swiglu_bwd) X(mi_wgrad_suits) X(mi_wgrad_workspace) X(mi_wgrad)
+  X(mi_swiglu_bwd) X(mi_wgrad_suits) X(mi_wgrad_workspace) X(mi_wgrad)                     \
+  X(mi_rotary_qk) X(mi_qk_norm_rotary) X(mi_qk_norm_rotary_workspace)                      \
+  X(mi_qk_norm_rotary_bwd) X(mi_sattn_tiles) X(mi_sattn_fwd) X(mi_sattn_bwd_workspace)     \
+  X(mi_sattn_bwd) X(mi_decode_workspace) X(mi_decode_attn)
 
 struct Bound {
 #define X(f) decltype(&::f) f = nullptr;
@@ -619,6 +624,329 @@ struct LinearGradInto : torch::autograd::Function<LinearGradInto> {
 };
 
 // ---------------------------------------------------------------------------
+// Rotary embedding at given positions, alone and behind the norm of each head
+// ---------------------------------------------------------------------------
+// A captured backward whose leaves still belong to an eager graph: their gradients
+// would go to the stream of that graph, from inside the capture, which invalidates
+// it and ends the process.  Noted in the forward (where the leaves are at hand),
+// refused in the backward.
+bool capturing(const Tensor& t) {
+  const c10::DeviceGuard guard(t.device());
+  return c10::hip::currentStreamCaptureStatusMayInitCtx() != c10::hip::CaptureStatus::None;
+}
+void note_leaves(AutogradContext* ctx, std::initializer_list<Tensor> inputs) {
+  const Tensor& first = *inputs.begin();
+  if (!capturing(first)) return;
+  const c10::Stream now =
+      c10::impl::VirtualGuardImpl(first.device().type()).getStream(first.device());
+  for (const Tensor& t : inputs) {
+    if (!t.is_leaf() || !t.requires_grad()) continue;
+    const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
+    if (leaf && leaf->stream() && *leaf->stream() != now) ctx->saved_data["eager_leaf"] = true;
+  }
+}
+void check_leaves(AutogradContext* ctx, const Tensor& grad) {
+  TORCH_CHECK(!ctx->saved_data.count("eager_leaf") || !capturing(grad),
+              "backward captured into a graph while an eager graph of the same leaf tensors is "
+              "alive: drop or detach its outputs first");
+}
+
+struct Angles {
+  Tensor cos, sin, pos;  // pos may be undefined
+  bool interleaved;
+};
+
+bool angles_ok(const Tensor& q, const Tensor& k, const Angles& r) {
+  if (q.dim() != 4 || k.dim() != 4 || q.size(0) != k.size(0) || q.size(1) != k.size(1) ||
+      q.size(3) != k.size(3) || code(q) < 0 || q.scalar_type() != k.scalar_type() ||
+      r.cos.dim() != 2 || r.cos.sizes() != r.sin.sizes() || code(r.cos) < 0 ||
+      r.cos.scalar_type() != r.sin.scalar_type() || 2 * r.cos.size(1) > q.size(3) ||
+      !one_device(q, k, r.cos, r.sin))
+    return false;
+  for (int64_t i = 0; i < 4; ++i)
+    if (q.size(i) >= 1ll << 31 || k.size(i) >= 1ll << 31) return false;
+  if (!r.pos.defined()) return r.cos.size(0) >= q.size(0);
+  return (r.pos.scalar_type() == at::kLong || r.pos.scalar_type() == at::kInt) &&
+         one_device(q, r.pos) && (r.pos.dim() == 1 || r.pos.dim() == 2) &&
+         r.pos.size(0) == q.size(0) && (r.pos.dim() == 1 || r.pos.size(1) == q.size(1));
+}
+
+mi_rotary rotary_how(const Tensor& q, const Tensor& k, const Angles& r) {
+  mi_rotary h = {};
+  h.tab_dtype = dt(r.cos);
+  h.S = q.size(0); h.B = q.size(1); h.H = q.size(2); h.Hk = k.size(2); h.D = q.size(3);
+  h.R = 2 * r.cos.size(1);
+  h.interleaved = r.interleaved;
+  h.cos_tab = r.cos.data_ptr();
+  h.sin_tab = r.sin.data_ptr();
+  for (int i = 0; i < 2; ++i) {
+    h.cos_strides[i] = r.cos.stride(i);
+    h.sin_strides[i] = r.sin.stride(i);
+  }
+  h.table_rows = r.cos.size(0);
+  if (r.pos.defined()) {
+    h.positions = r.pos.data_ptr();
+    h.pos_strides[0] = r.pos.stride(0);
+    h.pos_strides[1] = r.pos.dim() == 2 ? r.pos.stride(1) : 0;
+    h.pos_bytes = r.pos.element_size();
+  }
+  return h;
+}
+
+// What a backward gets: gradients of q's and k's sizes and dtype, tables that fit.
+void check_rotary_grads(const Tensor& gq, const Tensor& gk, const Angles& r) {
+  TORCH_CHECK_VALUE(angles_ok(gq, gk, r), "gradients and saved cos / sin / positions do not fit");
+}
+
+struct RotaryQK : torch::autograd::Function<RotaryQK> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const Angles& r) {
+    const c10::DeviceGuard guard(q.device());
+    Tensor qo = empty(q.sizes(), q), ko = empty(k.sizes(), k);
+    const mi_rotary h = rotary_how(q, k, r);
+    check(lib.mi_rotary_qk(dt(q), &h, 0, q.data_ptr(), q.strides().data(), k.data_ptr(),
+                           k.strides().data(), qo.data_ptr(), qo.strides().data(), ko.data_ptr(),
+                           ko.strides().data(), stream(q)),
+          "mi_rotary_qk");
+    ctx->save_for_backward({r.cos, r.sin, r.pos});
+    note_leaves(ctx, {q, k});
+    ctx->saved_data["interleaved"] = r.interleaved;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Angles r{s[0], s[1], s[2], ctx->saved_data["interleaved"].toBool()};
+    const Tensor &gq = grads[0], &gk = grads[1];
+    check_leaves(ctx, gq);
+    check_rotary_grads(gq, gk, r);
+    const c10::DeviceGuard guard(gq.device());
+    Tensor dq = empty(gq.sizes(), gq), dk = empty(gk.sizes(), gk);
+    const mi_rotary h = rotary_how(gq, gk, r);
+    check(lib.mi_rotary_qk(dt(gq), &h, 1, gq.data_ptr(), gq.strides().data(), gk.data_ptr(),
+                           gk.strides().data(), dq.data_ptr(), dq.strides().data(), dk.data_ptr(),
+                           dk.strides().data(), stream(gq)),
+          "mi_rotary_qk");
+    return {dq, dk, Tensor()};
+  }
+};
+
+struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                               const Tensor& wq_, const Tensor& wk_, double eps, const Angles& r) {
+    const c10::DeviceGuard guard(q.device());
+    const Tensor wq = wq_.contiguous(), wk = wk_.contiguous();
+    Tensor qo = empty(q.sizes(), q), ko = empty(k.sizes(), k);
+    const mi_rotary h = rotary_how(q, k, r);
+    check(lib.mi_qk_norm_rotary(dt(q), dt(wq), &h, eps, q.data_ptr(), q.strides().data(),
+                                k.data_ptr(), k.strides().data(), wq.data_ptr(), wk.data_ptr(),
+                                qo.data_ptr(), qo.strides().data(), ko.data_ptr(),
+                                ko.strides().data(), stream(q)),
+          "mi_qk_norm_rotary");
+    ctx->save_for_backward({q, k, wq, wk, r.cos, r.sin, r.pos});
+    note_leaves(ctx, {q, k, wq_, wk_});
+    ctx->saved_data["interleaved"] = r.interleaved;
+    ctx->saved_data["eps"] = eps;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &wq = s[2], &wk = s[3];
+    const Angles r{s[4], s[5], s[6], ctx->saved_data["interleaved"].toBool()};
+    const Tensor &gq = grads[0], &gk = grads[1];
+    check_leaves(ctx, gq);
+    check_rotary_grads(gq, gk, r);
+    strided("saved q", q, gq.sizes(), gq.scalar_type(), gq);
+    strided("saved k", k, gk.sizes(), gk.scalar_type(), gk);
+    dense("weight of q", wq, {gq.size(3)}, wq.scalar_type(), gq);
+    dense("weight of k", wk, {gq.size(3)}, wq.scalar_type(), gq);
+    TORCH_CHECK_VALUE(code(wq) >= 0, "saved weights of dtype ", wq.scalar_type());
+    const c10::DeviceGuard guard(gq.device());
+    Tensor dq = empty(gq.sizes(), gq), dk = empty(gk.sizes(), gk);
+    Tensor dwq = empty(wq.sizes(), wq), dwk = empty(wk.sizes(), wk);
+    const mi_rotary h = rotary_how(gq, gk, r);
+    const int64_t n = lib.mi_qk_norm_rotary_workspace(&h);
+    Tensor ws = empty_f32({n}, gq);
+    check(lib.mi_qk_norm_rotary_bwd(
+              dt(gq), dt(wq), &h, ctx->saved_data["eps"].toDouble(), q.data_ptr(),
+              q.strides().data(), k.data_ptr(), k.strides().data(), wq.data_ptr(), wk.data_ptr(),
+              gq.data_ptr(), gq.strides().data(), gk.data_ptr(), gk.strides().data(),
+              dq.data_ptr(), dq.strides().data(), dk.data_ptr(), dk.strides().data(),
+              dwq.data_ptr(), dwk.data_ptr(), ws.data_ptr<float>(), n, stream(gq)),
+          "mi_qk_norm_rotary_bwd");
+    return {dq, dk, dwq, dwk, Tensor(), Tensor()};
+  }
+};
+
+// ---------------------------------------------------------------------------
+// Attention with modified scores
+// ---------------------------------------------------------------------------
+struct Mods {
+  bool causal;
+  double cap, scale;
+  Tensor slopes, docs, prefix;  // may be undefined
+};
+
+// A size-1 dim's stride addresses nothing: 0, so that it does not spoil alignment.
+struct Strides {
+  int64_t s[4];
+  explicit Strides(const Tensor& t) {
+    for (int64_t i = 0; i < t.dim(); ++i) s[i] = t.size(i) == 1 && i + 1 < t.dim() ? 0 : t.stride(i);
+  }
+};
+// t, or a copy whose rows are 16-byte aligned with unit stride and less than 8 MB apart.
+Tensor rows_ready(const Tensor& t) {
+  const Strides st(t);
+  const int64_t e = t.element_size(), last = t.dim() - 1;
+  bool ok = t.stride(last) == 1 && (uintptr_t)t.data_ptr() % 16 == 0;
+  for (int64_t i = 0; i < last; ++i)
+    ok = ok && st.s[i] * e % 16 == 0 && (i + 1 < last || st.s[i] * e * 256 < 1ll << 31);
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
+}
+
+bool mods_ok(const Tensor& q, const Mods& m, int64_t B, int64_t H, int64_t Sk) {
+  if (m.slopes.defined() &&
+      (m.slopes.scalar_type() != at::kFloat || m.slopes.dim() != 1 || m.slopes.size(0) != H ||
+       !one_device(q, m.slopes) || (m.slopes.requires_grad() && at::GradMode::is_enabled())))
+    return false;
+  if (m.docs.defined() &&
+      (m.docs.scalar_type() != at::kInt || m.docs.dim() != 2 || m.docs.size(0) != B ||
+       m.docs.size(1) != Sk || !one_device(q, m.docs)))
+    return false;
+  return !m.prefix.defined() ||
+         (m.causal && m.prefix.scalar_type() == at::kInt && m.prefix.dim() == 1 &&
+          m.prefix.size(0) == B && one_device(q, m.prefix));
+}
+
+bool sattn_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Mods& m) {
+  return q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
+         q.size(3) == k.size(3) && q.size(1) % k.size(1) == 0 && q.size(2) <= k.size(2) &&
+         code(q) >= 0 && q.scalar_type() == k.scalar_type() &&
+         q.scalar_type() == v.scalar_type() && one_device(q, k, v) && q.size(3) % 8 == 0 &&
+         q.size(3) <= 128 && k.size(2) <= 1 << 24 && q.size(0) < 1ll << 31 &&
+         q.size(1) < 1ll << 31 && mods_ok(q, m, q.size(0), q.size(1), k.size(2));
+}
+
+mi_score_mods c_mods(const Mods& m) {
+  mi_score_mods c = {};
+  c.causal = m.causal;
+  c.softcap = m.cap;
+  c.slopes = m.slopes.defined() ? m.slopes.data_ptr<float>() : nullptr;
+  c.document_ids = m.docs.defined() ? m.docs.data_ptr<int32_t>() : nullptr;
+  c.prefix_lens = m.prefix.defined() ? m.prefix.data_ptr<int32_t>() : nullptr;
+  return c;
+}
+
+Mods dense_mods(const Mods& m) {
+  auto c = [](const Tensor& t) { return t.defined() ? t.contiguous() : t; };
+  return {m.causal, m.cap, m.scale, c(m.slopes), c(m.docs), c(m.prefix)};
+}
+
+struct SAttnOut {
+  Tensor o, lse, tiles;
+};
+// q, k, v by rows_ready, m by dense_mods.
+SAttnOut sattn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Mods& m) {
+  const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1),
+                Sk = k.size(2);
+  SAttnOut r{empty({B, H, Sq, D}, q), empty_f32({B, H, Sq}, q), Tensor()};
+  if (m.docs.defined())
+    r.tiles = at::empty({lib.mi_sattn_tiles(B, Sq, Sk)}, q.options().dtype(at::kInt));
+  const mi_score_mods c = c_mods(m);
+  check(lib.mi_sattn_fwd(dt(q), B, H, Hk, Sq, Sk, D, m.scale, &c, q.data_ptr(), Strides(q).s,
+                         k.data_ptr(), Strides(k).s, v.data_ptr(), Strides(v).s, r.o.data_ptr(),
+                         Strides(r.o).s, r.lse.data_ptr<float>(),
+                         r.tiles.defined() ? r.tiles.data_ptr<int32_t>() : nullptr, stream(q)),
+        "mi_sattn_fwd");
+  return r;
+}
+
+struct ScoredAttn : torch::autograd::Function<ScoredAttn> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_,
+                        const Mods& m_) {
+    const c10::DeviceGuard guard(q_.device());
+    const Tensor q = rows_ready(q_), k = rows_ready(k_), v = rows_ready(v_);
+    const Mods m = dense_mods(m_);
+    const SAttnOut r = sattn_fwd(q, k, v, m);
+    ctx->save_for_backward({q, k, v, r.o, r.lse, r.tiles, m.slopes, m.docs, m.prefix});
+    ctx->saved_data["causal"] = m.causal;
+    ctx->saved_data["cap"] = m.cap;
+    ctx->saved_data["scale"] = m.scale;
+    note_leaves(ctx, {q_, k_, v_});
+    return r.o;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &tiles = s[5];
+    const Mods m{ctx->saved_data["causal"].toBool(), ctx->saved_data["cap"].toDouble(),
+                 ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8]};
+    check_leaves(ctx, grads[0]);
+    const Tensor go = rows_ready(grads[0]);
+    const c10::DeviceGuard guard(go.device());
+    strided("saved q", q, go.sizes(), go.scalar_type(), go);
+    TORCH_CHECK_VALUE(sattn_ok(q, k, v, m), "saved tensors do not fit each other");
+    const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1),
+                  Sk = k.size(2);
+    dense("output", o, {B, H, Sq, D}, q.scalar_type(), q);
+    dense("lse", lse, {B, H, Sq}, at::kFloat, q);
+    if (m.slopes.defined()) dense("slopes", m.slopes, {H}, at::kFloat, q);
+    if (m.prefix.defined()) dense("prefix_lens", m.prefix, {B}, at::kInt, q);
+    if (m.docs.defined()) {
+      dense("document_ids", m.docs, {B, Sk}, at::kInt, q);
+      dense("document tiles", tiles, {lib.mi_sattn_tiles(B, Sq, Sk)}, at::kInt, q);
+    }
+    const int64_t n = lib.mi_sattn_bwd_workspace(dt(q), B, H, Hk, Sq, Sk, D);
+    Tensor ws = empty_f32({n}, q);
+    Tensor dq = empty({B, H, Sq, D}, q), dk = empty({B, Hk, Sk, D}, q),
+           dv = empty({B, Hk, Sk, D}, q);
+    const mi_score_mods c = c_mods(m);
+    check(lib.mi_sattn_bwd(dt(q), B, H, Hk, Sq, Sk, D, m.scale, &c, q.data_ptr(), Strides(q).s,
+                           k.data_ptr(), Strides(k).s, v.data_ptr(), Strides(v).s, o.data_ptr(),
+                           Strides(o).s, go.data_ptr(), Strides(go).s, lse.data_ptr<float>(),
+                           tiles.defined() ? tiles.data_ptr<int32_t>() : nullptr,
+                           ws.data_ptr<float>(), n, dq.data_ptr(), Strides(dq).s, dk.data_ptr(),
+                           Strides(dk).s, dv.data_ptr(), Strides(dv).s, stream(q)),
+          "mi_sattn_bwd");
+    return {dq, dk, dv, Tensor()};
+  }
+};
+
+bool decode_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& lengths,
+               const Mods& m) {
+  if (q.dim() != 3 || k.dim() != 4 || k.sizes() != v.sizes() || q.size(0) != k.size(0) ||
+      q.size(2) != k.size(3) || q.size(1) % k.size(1) || code(q) < 0 ||
+      q.scalar_type() != k.scalar_type() || q.scalar_type() != v.scalar_type() ||
+      !one_device(q, k, v) || q.size(2) % 8 || q.size(2) > 128 || k.size(2) > 1 << 24 ||
+      q.size(0) >= 1ll << 31 || q.size(1) >= 1ll << 31)
+    return false;
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad()))
+    return false;
+  if (lengths.defined() && (lengths.scalar_type() != at::kInt || lengths.dim() != 1 ||
+                            lengths.size(0) != q.size(0) || !one_device(q, lengths)))
+    return false;
+  return mods_ok(q, m, q.size(0), q.size(1), k.size(2));
+}
+
+Tensor decode(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& lengths_,
+              const Mods& m_) {
+  const c10::DeviceGuard guard(q_.device());
+  const Tensor q = rows_ready(q_), k = rows_ready(k_), v = rows_ready(v_);
+  const Mods m = dense_mods(m_);
+  const Tensor lengths = lengths_.defined() ? lengths_.contiguous() : lengths_;
+  const int64_t B = q.size(0), H = q.size(1), D = q.size(2), Hk = k.size(1), S = k.size(2);
+  Tensor o = empty({B, H, D}, q);
+  const int64_t n = lib.mi_decode_workspace(dt(q), B, H, Hk, S, D);
+  Tensor ws = n ? empty_f32({n}, q) : Tensor();
+  check(lib.mi_decode_attn(dt(q), B, H, Hk, S, D, m.scale, m.cap,
+                           m.slopes.defined() ? m.slopes.data_ptr<float>() : nullptr,
+                           lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr,
+                           q.data_ptr(), Strides(q).s, k.data_ptr(), Strides(k).s, v.data_ptr(),
+                           Strides(v).s, o.data_ptr(), Strides(o).s,
+                           n ? ws.data_ptr<float>() : nullptr, n, stream(q)),
+        "mi_decode_attn");
+  return o;
+}
+
+// ---------------------------------------------------------------------------
 // The module's functions: None for a call that is not plain
 // ---------------------------------------------------------------------------
 using Args = PyObject* const*;
@@ -773,6 +1101,95 @@ PyObject* py_linear_into_grad(PyObject*, Args a, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// None (t stays undefined) or a plain tensor.
+bool plain_or_none(PyObject* o, Tensor& t) { return o == Py_None || plain(o, t); }
+
+// a[0] q, a[1] k, ..., a[i] cos, a[i + 1] sin, a[i + 2] positions, a[i + 3] interleaved
+bool angles(Args a, int i, Angles& r) {
+  return plain(a[i], r.cos) && plain(a[i + 1], r.sin) && plain_or_none(a[i + 2], r.pos) &&
+         truth(a[i + 3], r.interleaved);
+}
+
+PyObject* py_rotary_qk(PyObject*, Args a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k;
+  Angles r;
+  PLAIN(n == 6 && plain(a[0], q) && plain(a[1], k) && angles(a, 2, r) && plain_context() &&
+        angles_ok(q, k, r));
+  const variable_list y = released([&] { return RotaryQK::apply(q, k, r); });
+  return pair(y[0], y[1]);
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_qk_norm_rotary(PyObject*, Args a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, wq, wk;
+  Angles r;
+  double eps;
+  PLAIN(n == 9 && plain(a[0], q) && plain(a[1], k) && plain(a[2], wq) && plain(a[3], wk) &&
+        angles(a, 4, r) && number(a[8], eps) && plain_context() && angles_ok(q, k, r) &&
+        wq.dim() == 1 && wq.size(0) == q.size(3) && wq.sizes() == wk.sizes() && code(wq) >= 0 &&
+        wq.scalar_type() == wk.scalar_type() && one_device(q, wq, wk) && q.size(3) <= 512);
+  const variable_list y = released([&] { return QKNormRotary::apply(q, k, wq, wk, eps, r); });
+  return pair(y[0], y[1]);
+  END_HANDLE_TH_ERRORS
+}
+
+// Softcap (None: 0) and scale (None: 1 / sqrt(D)), both as the C ABI wants them.
+bool cap_and_scale(PyObject* cap, PyObject* scale, int64_t D, Mods& m) {
+  m.cap = 0.0;
+  m.scale = 1.0 / std::sqrt((double)D);
+  return (cap == Py_None || (number(cap, m.cap) && m.cap > 0.0)) &&
+         (scale == Py_None || number(scale, m.scale));
+}
+
+// q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale
+bool sattn_args(Args a, Py_ssize_t n, Tensor& q, Tensor& k, Tensor& v, Mods& m) {
+  return n == 9 && plain(a[0], q) && plain(a[1], k) && plain(a[2], v) && truth(a[3], m.causal) &&
+         plain_or_none(a[5], m.slopes) && plain_or_none(a[6], m.docs) &&
+         plain_or_none(a[7], m.prefix) && plain_context() && sattn_ok(q, k, v, m) &&
+         cap_and_scale(a[4], a[8], q.size(3), m);
+}
+
+PyObject* py_scored_attn(PyObject*, Args a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v;
+  Mods m;
+  PLAIN(sattn_args(a, n, q, k, v, m));
+  return THPVariable_Wrap(released([&] { return ScoredAttn::apply(q, k, v, m); }));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_scored_attn_forward(PyObject*, Args a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v;
+  Mods m;
+  PLAIN(sattn_args(a, n, q, k, v, m));
+  const SAttnOut r = released([&] {
+    const c10::DeviceGuard guard(q.device());
+    const at::NoGradGuard no_grad;
+    return sattn_fwd(rows_ready(q), rows_ready(k), rows_ready(v), dense_mods(m));
+  });
+  return pair(r.o, r.lse);
+  END_HANDLE_TH_ERRORS
+}
+
+// q, k, v, lengths, softcap, slopes, scale
+PyObject* py_decode_attn(PyObject*, Args a, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  Tensor q, k, v, lengths;
+  Mods m;
+  m.causal = true;
+  PLAIN(n == 7 && plain(a[0], q) && plain(a[1], k) && plain(a[2], v) &&
+        plain_or_none(a[3], lengths) && plain_or_none(a[5], m.slopes) && plain_context() &&
+        decode_ok(q, k, v, lengths, m) && cap_and_scale(a[4], a[6], q.size(2), m));
+  return THPVariable_Wrap(released([&] {
+    const at::NoGradGuard no_grad;
+    return decode(q, k, v, lengths, m);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
 // bind({name: address}, MiError)
 PyObject* py_bind(PyObject*, Args a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -797,7 +1214,9 @@ PyObject* py_bind(PyObject*, Args a, Py_ssize_t n) {
 PyMethodDef methods[] = {FN(bind),       FN(flash_attn),  FN(flash_attn_forward),
                          FN(attention_block), FN(rope),   FN(rope_qk),
                          FN(xent),       FN(rms_norm),    FN(add_rms_norm),
-                         FN(swiglu),     FN(linear_into_grad), {nullptr, nullptr, 0, nullptr}};
+                         FN(swiglu),     FN(linear_into_grad), FN(rotary_qk),
+                         FN(qk_norm_rotary), FN(scored_attn), FN(scored_attn_forward),
+                         FN(decode_attn), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_torch_ops", nullptr, -1, methods};
 
 }  // namespace

@@ -470,6 +470,145 @@ mi_status mi_attn_bwd_noalloc(mi_dtype dtype, int B, int H, int S, int D, int ca
                               void* dv, const int64_t dv_strides[4],
                               void* stream);
 
+/*
+ * Rotary embedding of query and key heads, in the forms mi_rope_qk does not
+ * have.  q is [S, B, H, D], k [S, B, Hk, D] (four element strides each, any
+ * values), H and Hk independent.  The first R elements of each head are turned
+ * (R even, 2 <= R <= D), the others copied:
+ *   interleaved: pairs (2i, 2i + 1);  otherwise: pairs (i, i + R / 2)
+ *   (e, o) -> (e c - o s, e s + o c),  inverse: by the negated angle
+ * with c, s = cos / sin[position, i].  The tables have `table_rows` rows of R / 2
+ * angles (two element strides each).  positions: NULL (token s is at position s;
+ * table_rows >= S), or integers of pos_bytes (4 or 8) bytes read at
+ * s * pos_strides[0] + b * pos_strides[1]; a position that the tables do not have
+ * gives NaN in the turned elements and reads nothing out of bounds.  Computed in
+ * fp32, rounded once.  Outputs must not overlap inputs.  The reference's RoPE
+ * (core/rope_triton.py:10-148) is the interleaved form over whole heads at
+ * positions 0 .. S - 1 with H == Hk.
+ */
+typedef struct mi_rotary {
+  mi_dtype tab_dtype;
+  int S, B, H, Hk, D, R;
+  int interleaved;
+  const void* cos_tab;
+  const void* sin_tab;
+  int64_t cos_strides[2], sin_strides[2];
+  int64_t table_rows;
+  const void* positions;
+  int64_t pos_strides[2];
+  int pos_bytes;
+} mi_rotary;
+
+mi_status mi_rotary_qk(mi_dtype dtype, const mi_rotary* how, int inverse,
+                       const void* q, const int64_t q_strides[4],
+                       const void* k, const int64_t k_strides[4],
+                       void* q_out, const int64_t q_out_strides[4],
+                       void* k_out, const int64_t k_out_strides[4], void* stream);
+
+/*
+ * The same behind the RMSNorm of each head, in one pass:
+ *   n = x * rsqrt(mean(x^2) + eps) * w over the D elements, then the rotation of n,
+ * all in fp32, rounded once.  q_weight and k_weight: [D], dense, of w_dtype.
+ * D <= 512.  The outputs have the inputs' dtype.
+ */
+mi_status mi_qk_norm_rotary(mi_dtype dtype, mi_dtype w_dtype, const mi_rotary* how, float eps,
+                            const void* q, const int64_t q_strides[4],
+                            const void* k, const int64_t k_strides[4],
+                            const void* q_weight, const void* k_weight,
+                            void* q_out, const int64_t q_out_strides[4],
+                            void* k_out, const int64_t k_out_strides[4], void* stream);
+
+/*
+ * Backward of mi_qk_norm_rotary: gradients of q, k and both weights from those of
+ * the outputs.  q, k, weights and `how` as in the forward; dq, dk have the inputs'
+ * dtype, the weights' gradients w_dtype.  workspace:
+ * mi_qk_norm_rotary_workspace(how) floats, contents irrelevant.  The weights'
+ * gradients are summed in a fixed order.
+ */
+int64_t mi_qk_norm_rotary_workspace(const mi_rotary* how);
+mi_status mi_qk_norm_rotary_bwd(mi_dtype dtype, mi_dtype w_dtype, const mi_rotary* how, float eps,
+                                const void* q, const int64_t q_strides[4],
+                                const void* k, const int64_t k_strides[4],
+                                const void* q_weight, const void* k_weight,
+                                const void* dq_out, const int64_t dq_out_strides[4],
+                                const void* dk_out, const int64_t dk_out_strides[4],
+                                void* dq, const int64_t dq_strides[4],
+                                void* dk, const int64_t dk_strides[4],
+                                void* dq_weight, void* dk_weight, float* workspace,
+                                int64_t workspace_elems, void* stream);
+
+/*
+ * Attention with modified scores: queries [B, H, Sq, D] on keys and values
+ * [B, Hk, Sk, D], Sq <= Sk, H a multiple of Hk (query head h reads key head
+ * h / (H / Hk)).  The queries are the last Sq of the Sk positions.
+ *   z = scale q.k;  softcap > 0: z <- softcap * tanh(z / softcap)
+ *   slopes: z <- z - slopes[h] * |i - j|   (positions i of the query, j of the key)
+ *   key j is visible to query i iff
+ *     document_ids: id(i) == id(j) and id(i) >= 0 (a negative id is padding), and
+ *     causal:       j <= i, or j < prefix_lens[b]
+ *   O = softmax over the visible keys, times V;  lse = log sum exp of them
+ * A query without a visible key gets O = 0, lse = -inf and no gradient.  Keys and
+ * queries of negative id may hold anything, NaN included.
+ * D: a multiple of 8 up to 128.  bf16, f16 and fp32, all on matrix cores; every
+ * tensor has unit dim stride and 16-byte aligned rows.  Softmax statistics and
+ * sums are fp32.  The reference's attention (core/myFlashAttn.py:198-441) is the
+ * case H == Hk, Sq == Sk without any of these.
+ */
+typedef struct mi_score_mods {
+  int causal;
+  float softcap;               /* 0: none */
+  const float* slopes;         /* [H] or NULL */
+  const int32_t* document_ids; /* [B, Sk] dense or NULL */
+  const int32_t* prefix_lens;  /* [B] or NULL; with causal only */
+} mi_score_mods;
+
+/* int32 elements of `tiles` (16-byte aligned), which the forward fills where
+ * document_ids are given and the backward reads. */
+int64_t mi_sattn_tiles(int B, int Sq, int Sk);
+
+mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                       const mi_score_mods* mods,
+                       const void* q, const int64_t q_strides[4],
+                       const void* k, const int64_t k_strides[4],
+                       const void* v, const int64_t v_strides[4],
+                       void* o, const int64_t o_strides[4], float* lse /* [B, H, Sq] */,
+                       int32_t* tiles, void* stream);
+
+/* Floats of workspace that mi_sattn_bwd needs (16-byte aligned). */
+int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D);
+
+/* dQ [B, H, Sq, D], dK and dV [B, Hk, Sk, D] (summed over the query heads of each
+ * key head); no atomics: the same bits every time. */
+mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
+                       const mi_score_mods* mods,
+                       const void* q, const int64_t q_strides[4],
+                       const void* k, const int64_t k_strides[4],
+                       const void* v, const int64_t v_strides[4],
+                       const void* o, const int64_t o_strides[4],
+                       const void* dout, const int64_t dout_strides[4],
+                       const float* lse, const int32_t* tiles,
+                       float* workspace, int64_t workspace_elems,
+                       void* dq, const int64_t dq_strides[4],
+                       void* dk, const int64_t dk_strides[4],
+                       void* dv, const int64_t dv_strides[4], void* stream);
+
+/*
+ * The same for one new token of each sequence over its cache: q, o [B, H, D]
+ * (strides batch, head, dim), k and v [B, Hk, S, D].  The query is the last of the
+ * lengths[b] keys of sequence b (NULL: S of them); what lies behind them is never
+ * read, and lengths outside [0, S] are taken to the nearer end.  No keys: o = 0.
+ * softcap, slopes as above.  workspace: mi_decode_workspace(...) floats, contents
+ * irrelevant.
+ */
+int64_t mi_decode_workspace(mi_dtype dtype, int B, int H, int Hk, int S, int D);
+mi_status mi_decode_attn(mi_dtype dtype, int B, int H, int Hk, int S, int D, float scale,
+                         float softcap, const float* slopes, const int32_t* lengths,
+                         const void* q, const int64_t q_strides[3],
+                         const void* k, const int64_t k_strides[4],
+                         const void* v, const int64_t v_strides[4],
+                         void* o, const int64_t o_strides[3],
+                         float* workspace, int64_t workspace_elems, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
