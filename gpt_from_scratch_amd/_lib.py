@@ -31,7 +31,8 @@ EXPORTED = ("mi_version", "mi_status_str", "mi_last_error", "mi_attn_fwd", "mi_a
             "mi_rmsnorm_bwd_acc", "mi_rmsnorm_add_bwd_acc", "mi_copy_qk",
             "mi_wgrad_workspace", "mi_wgrad_suits", "mi_wgrad",
             "mi_rotary_qk", "mi_qk_norm_rotary", "mi_qk_norm_rotary_workspace",
-            "mi_qk_norm_rotary_bwd", "mi_sattn_tiles", "mi_sattn_fwd", "mi_sattn_bwd_workspace",
+            "mi_qk_norm_rotary_bwd", "mi_sattn_tiles", "mi_sattn_fwd_workspace", "mi_sattn_fwd",
+            "mi_sattn_bwd_workspace",
             "mi_sattn_bwd", "mi_decode_workspace", "mi_decode_attn")
 
 # B*H*S limit of mi_attn_bwd_noalloc (its static workspace array), include/mi_attn.h
@@ -149,12 +150,14 @@ def _declare(lib):
     lib.mi_sattn_tiles.restype = i64
     lib.mi_sattn_tiles.argtypes = [i, i, i]
     lib.mi_sattn_fwd.restype = i
-    lib.mi_sattn_fwd.argtypes = [i] * 7 + [f, mods, p, i64p, p, i64p, p, i64p, p, i64p, p, p, p]
+    lib.mi_sattn_fwd.argtypes = [i] * 7 + [f, mods] + [p, i64p] * 4 + [p, p, p, p, i64, p]
+    lib.mi_sattn_fwd_workspace.restype = i64
+    lib.mi_sattn_fwd_workspace.argtypes = [i] * 7
     lib.mi_sattn_bwd_workspace.restype = i64
     lib.mi_sattn_bwd_workspace.argtypes = [i] * 7
     lib.mi_sattn_bwd.restype = i
-    lib.mi_sattn_bwd.argtypes = [i] * 7 + [f, mods] + [p, i64p] * 5 + [p, p, p, i64] + \
-        [p, i64p] * 3 + [p]
+    lib.mi_sattn_bwd.argtypes = [i] * 7 + [f, mods] + [p, i64p] * 4 + [p, p, i64p] + \
+        [p, p, p, i64] + [p, i64p] * 3 + [p]
     lib.mi_decode_workspace.restype = i64
     lib.mi_decode_workspace.argtypes = [i] * 6
     lib.mi_decode_attn.restype = i
@@ -615,26 +618,30 @@ def sattn_tiles(q, k) -> int:
     return int(lib().mi_sattn_tiles(q.shape[0], q.shape[2], k.shape[2]))
 
 
-def sattn_fwd(q, k, v, mods, scale: float):
-    """Enqueue attention with modified scores: (o, lse, tiles) of q [B, H, Sq, D] and
-    k, v [B, Hk, Sk, D] by rows_ready; mods = (causal, softcap, slopes, docs, prefix),
-    dense tensors or None."""
+def sattn_fwd(q, k, v, mods, scale: float, grad: bool):
+    """Enqueue attention with modified scores: (o, o_lo, lse, tiles) of q [B, H, Sq, D]
+    and k, v [B, Hk, Sk, D] by rows_ready; mods = (causal, softcap, slopes, docs,
+    prefix), dense tensors or None.  o_lo (16-bit types, for `grad`): what rounding o
+    left."""
     _require_gpu(q, k, v, *(t for t in mods[2:] if t is not None))
     (B, H, Sq, D), (_, Hk, Sk, _) = q.shape, k.shape
     o = torch.empty(B, H, Sq, D, dtype=q.dtype, device=q.device)
+    o_lo = torch.empty_like(o) if grad and q.dtype != torch.float32 else None
     lse = torch.empty(B, H, Sq, dtype=torch.float32, device=q.device)
     tiles = None
     if mods[3] is not None:
         tiles = torch.empty(sattn_tiles(q, k), dtype=torch.int32, device=q.device)
+    n = lib().mi_sattn_fwd_workspace(dtype_code(q), B, H, Hk, Sq, Sk, D)
+    ws = torch.empty(n, dtype=torch.float32, device=q.device) if n else None
     st = lib().mi_sattn_fwd(dtype_code(q), B, H, Hk, Sq, Sk, D, float(scale), _score_mods(*mods),
                             _ptr(q), _row_strides(q), _ptr(k), _row_strides(k), _ptr(v),
-                            _row_strides(v), _ptr(o), _row_strides(o), _ptr(lse), _opt_ptr(tiles),
-                            _stream(q))
+                            _row_strides(v), _ptr(o), _row_strides(o), _opt_ptr(o_lo), _ptr(lse),
+                            _opt_ptr(tiles), _opt_ptr(ws), n, _stream(q))
     _check(st, "mi_sattn_fwd")
-    return o, lse, tiles
+    return o, o_lo, lse, tiles
 
 
-def sattn_bwd(q, k, v, o, do, lse, tiles, mods, scale: float):
+def sattn_bwd(q, k, v, o, o_lo, do, lse, tiles, mods, scale: float):
     """Enqueue the backward of sattn_fwd: (dq, dk, dv)."""
     _require_gpu(q, k, v, o, do, lse, *(t for t in mods[2:] if t is not None))
     (B, H, Sq, D), (_, Hk, Sk, _) = q.shape, k.shape
@@ -644,9 +651,10 @@ def sattn_bwd(q, k, v, o, do, lse, tiles, mods, scale: float):
     dk, dv = (torch.empty(k.shape, dtype=q.dtype, device=q.device) for _ in range(2))
     st = lib().mi_sattn_bwd(dtype_code(q), B, H, Hk, Sq, Sk, D, float(scale), _score_mods(*mods),
                             _ptr(q), _row_strides(q), _ptr(k), _row_strides(k), _ptr(v),
-                            _row_strides(v), _ptr(o), _row_strides(o), _ptr(do), _row_strides(do),
-                            _ptr(lse), _opt_ptr(tiles), _ptr(ws), n, _ptr(dq), _row_strides(dq),
-                            _ptr(dk), _row_strides(dk), _ptr(dv), _row_strides(dv), _stream(q))
+                            _row_strides(v), _ptr(o), _row_strides(o), _opt_ptr(o_lo), _ptr(do),
+                            _row_strides(do), _ptr(lse), _opt_ptr(tiles), _ptr(ws), n, _ptr(dq),
+                            _row_strides(dq), _ptr(dk), _row_strides(dk), _ptr(dv),
+                            _row_strides(dv), _stream(q))
     _check(st, "mi_sattn_bwd")
     return dq, dk, dv
 

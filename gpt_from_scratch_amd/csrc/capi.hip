@@ -1361,6 +1361,16 @@ mi_status check_mods(const mi_score_mods* m, const int32_t* tiles) {
   return MI_OK;
 }
 
+mi_status check_workspace(const float* ws, int64_t have, int64_t want) {
+  if (want == 0) return MI_OK;
+  if (ws == nullptr || ((uintptr_t)ws) % 16)
+    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: 16-byte aligned memory wanted");
+  if (have < want)
+    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted", (long long)have,
+                (long long)want);
+  return MI_OK;
+}
+
 mi::ScoreConst score_const(float scale, float softcap) {
   mi::ScoreConst c = {};
   c.c = scale * 1.4426950408889634f;
@@ -1401,8 +1411,9 @@ int64_t mi_sattn_tiles(int B, int Sq, int Sk) {
 mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
                        const mi_score_mods* mods, const void* q, const int64_t q_strides[4],
                        const void* k, const int64_t k_strides[4], const void* v,
-                       const int64_t v_strides[4], void* o, const int64_t o_strides[4], float* lse,
-                       int32_t* tiles, void* stream) {
+                       const int64_t v_strides[4], void* o, const int64_t o_strides[4], void* o_lo,
+                       float* lse, int32_t* tiles, float* workspace, int64_t workspace_elems,
+                       void* stream) {
   MI_SOLE_COPY();
   mi_status st;
   if ((st = check_mods(mods, tiles)) != MI_OK) return st;
@@ -1416,7 +1427,12 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
   a.k = targ(k, k_strides);
   a.v = targ(v, v_strides);
   a.o = targ(o, o_strides);
+  a.olo = o_lo;
   a.lse = lse;
+  if (((uintptr_t)o_lo) % 16) return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-byte aligned rows wanted");
+  if ((st = check_workspace(workspace, workspace_elems, mi::sattn_fwd_workspace(a))) != MI_OK)
+    return st;
+  mi::sattn_fwd_split(a, workspace);
   if (a.docs) {
     st = launched(mi::launch_doc_tiles(a.docs, tiles, B, Sq, Sk, (hipStream_t)stream), "doc_tiles");
     if (st != MI_OK) return st;
@@ -1425,16 +1441,24 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
                   "sattn_fwd");
 }
 
+int64_t mi_sattn_fwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
+  if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
+  return mi::sattn_fwd_workspace(sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr));
+}
+
 int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
   if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
-  return 2 * (int64_t)B * H * Sq;
+  mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr);
+  int64_t n = 0;
+  mi::sattn_bwd_split(a, nullptr, &n);
+  return n;
 }
 
 mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
                        const mi_score_mods* mods, const void* q, const int64_t q_strides[4],
                        const void* k, const int64_t k_strides[4], const void* v,
                        const int64_t v_strides[4], const void* o, const int64_t o_strides[4],
-                       const void* dout, const int64_t dout_strides[4], const float* lse,
+                       const void* o_lo, const void* dout, const int64_t dout_strides[4], const float* lse,
                        const int32_t* tiles, float* workspace, int64_t workspace_elems, void* dq,
                        const int64_t dq_strides[4], void* dk, const int64_t dk_strides[4],
                        void* dv, const int64_t dv_strides[4], void* stream) {
@@ -1446,21 +1470,11 @@ mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
                                  {dout, dout_strides}, {dq, dq_strides}, {dk, dk_strides},
                                  {dv, dv_strides}})) != MI_OK)
     return st;
-  if (lse == nullptr || workspace == nullptr || ((uintptr_t)workspace) % 16)
-    return fail(MI_ERR_INVALID_ARGUMENT, "lse / workspace: 16-byte aligned memory wanted");
-  const int64_t want = mi_sattn_bwd_workspace(dtype, B, H, Hk, Sq, Sk, D);
-  if (workspace_elems < want)
-    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted",
-                (long long)workspace_elems, (long long)want);
-  // delta and lse * log2(e), as for the attention without modified scores
-  mi::AttnArgs pre = {};
-  pre.o = targ(o, o_strides);
-  pre.dout = targ(dout, dout_strides);
-  pre.lse = const_cast<float*>(lse);
-  pre.delta = workspace;
-  pre.B = B; pre.H = H; pre.S = Sq; pre.D = D;
-  st = launched(mi::launch_attn_delta(dtype, pre, (hipStream_t)stream), "attn_delta");
-  if (st != MI_OK) return st;
+  if (lse == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "lse: null pointer");
+  if (((uintptr_t)o_lo) % 16) return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-byte aligned rows wanted");
+  if ((st = check_workspace(workspace, workspace_elems,
+                            mi_sattn_bwd_workspace(dtype, B, H, Hk, Sq, Sk, D))) != MI_OK)
+    return st;
   mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, scale, *mods, tiles);
   a.q = targ(q, q_strides);
   a.k = targ(k, k_strides);
@@ -1469,8 +1483,10 @@ mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
   a.dq = targ(dq, dq_strides);
   a.dk = targ(dk, dk_strides);
   a.dv = targ(dv, dv_strides);
-  a.delta = workspace;
-  a.lse2 = workspace + (int64_t)B * H * Sq;
+  a.o = targ(o, o_strides);
+  a.olo = const_cast<void*>(o_lo);
+  a.lse = const_cast<float*>(lse);
+  mi::sattn_bwd_split(a, workspace, nullptr);
   return launched(mi::launch_sattn_bwd(dtype, a, mods->softcap > 0.f, (hipStream_t)stream),
                   "sattn_bwd");
 }
@@ -1498,9 +1514,7 @@ mi_status mi_decode_attn(mi_dtype dtype, int B, int H, int Hk, int S, int D, flo
   if (((uintptr_t)q) % 16 || q_strides[0] * esz % 16 || q_strides[1] * esz % 16)
     return fail(MI_ERR_UNSUPPORTED, "rows must be 16-byte aligned");
   const int64_t want = mi_decode_workspace(dtype, B, H, Hk, S, D);
-  if (want && (workspace == nullptr || workspace_elems < want))
-    return fail(MI_ERR_INVALID_ARGUMENT, "workspace: %lld elements, %lld wanted",
-                (long long)workspace_elems, (long long)want);
+  if ((st = check_workspace(workspace, workspace_elems, want)) != MI_OK) return st;
   mi::DecodeArgs a = {};
   a.q = q;
   a.q_sb = q_strides[0]; a.q_sh = q_strides[1];

@@ -1,20 +1,25 @@
 // sattn_bwd.hip — backward of attention with modified scores, for bf16, f16 and
-// fp32 (sattn_device.h has the forward's mathematics).  With lse and
-// delta = rowsum(dO * O) from before (attn_delta):
+// fp32 (sattn_device.h has the forward's mathematics).  With lse from before and
+// delta = rowsum(dO * O):
 //   P = exp(x - lse);  dV = P^T dO;  dP = dO V^T;  dx = P * (dP - delta)
 //   dz = dx * (1 - tanh^2(z / cap));  dQ = scale * dz K;  dK = scale * dz^T Q
 // dK and dV of a key head sum over the query heads that share it.
 //
-// Two kinds of workgroup, as in attn_bwd.hip, both without atomics, so results
-// repeat bit for bit:
+// Two kinds of work item in one launch, as in attn_bwd.hip, both without atomics,
+// so results repeat bit for bit:
 //   dK/dV: 128 keys of one key head, looping over the group's query heads and
 //     their query tiles; S = Q K^T and dP = dO V^T keep a key per lane, so P and
 //     dz feed dV^T = dO^T P and dK^T = Q^T dz from the accumulators.  The dP
 //     accumulators start at +delta and V is negated, so they end at delta - dP;
 //   dQ: 128 queries of one head, looping over key tiles; a query per lane.
-// Five products in dK/dV and dQ together recompute S and dP once each more than
-// the least: 7 products against 5, in exchange for no atomics on dQ.
-// Tiles without a visible pair are not visited, as in the forward (TileScan).
+// S and dP are formed twice, 7 products where 5 would do, in exchange for no
+// atomics on dQ.  Tiles without a visible pair are not visited, as in the forward
+// (tile_walk).  An item that would be too long a chain for the size of the launch is
+// split into parts (bwd_parts), whose fp32 sums a last launch adds up in order.
+//
+// delta subtracts from dP what O says, so O's rounding would reach every dz of a
+// row: the forward keeps what the rounding left (olo), and delta is as exact as fp32
+// sums are.
 #include <type_traits>
 
 #include "sattn_device.h"
@@ -60,27 +65,70 @@ __device__ __forceinline__ float prob(float s, float dist, float slope2, float l
 }
 
 // ---------------------------------------------------------------------------
+// delta and lse * log2(e)
+// ---------------------------------------------------------------------------
+// Eight lanes per row of 16-byte chunks.
+template <typename E>
+__global__ __launch_bounds__(256) void sattn_delta_kernel(SAttnArgs a, uint32_t rows) {
+  constexpr int ESZ = Elem<E>::kBytes;
+  const uint32_t row = blockIdx.x * 32u + threadIdx.x / 8;
+  const int sub = threadIdx.x % 8;
+  float sum = 0.f;
+  if (row < rows) {
+    const uint32_t bh = row / a.Sq, s = row - bh * a.Sq, b = bh / a.H, h = bh - b * a.H;
+    const int64_t at = (b * a.o.sb + h * a.o.sh + s * a.o.ss) * ESZ;
+    const u32x4* o = (const u32x4*)((const char*)a.o.ptr + at);
+    const u32x4* lo = a.olo ? (const u32x4*)((const char*)a.olo + at) : nullptr;
+    const u32x4* d = (const u32x4*)((const char*)a.dout.ptr +
+                                    (b * a.dout.sb + h * a.dout.sh + s * a.dout.ss) * ESZ);
+    for (int c = sub; c < a.dch; c += 8) {
+      const u32x4 x = o[c], y = d[c], z = lo ? lo[c] : u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (ESZ == 4) {
+          sum = __builtin_fmaf(__uint_as_float(x[i]), __uint_as_float(y[i]), sum);
+        } else {
+          sum = __builtin_fmaf(E::to_f32(x[i] & 0xffff) + E::to_f32(z[i] & 0xffff),
+                               E::to_f32(y[i] & 0xffff), sum);
+          sum = __builtin_fmaf(E::to_f32(x[i] >> 16) + E::to_f32(z[i] >> 16),
+                               E::to_f32(y[i] >> 16), sum);
+        }
+      }
+    }
+  }
+  sum = group_sum<8>(sum);
+  if (row < rows && sub == 0) {
+    const_cast<float*>(a.delta)[row] = sum;
+    const_cast<float*>(a.lse2)[row] = a.lse[row] * kLog2e;
+  }
+}
+
+// ---------------------------------------------------------------------------
 // dK, dV
 // ---------------------------------------------------------------------------
+// Two tiles of each streamed tensor, per-row values of the queries, own rows of K.
+struct Buffers {
+  char *A0, *A1, *B0, *B1;
+  float *S0, *S1;  // lse2, delta, document ids; for dQ: document ids
+  char* own;
+  int* list;       // see tile_walk
+};
+
 template <typename E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(SAttnArgs a) {
+__device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Buffers& buf) {
   using L = Lay<E, D>;
   constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
   constexpr bool K_IN_LDS = L::RB > 128;  // K and V rows and both sums pass 256 registers
-  __shared__ __attribute__((aligned(16))) char Q0[T * L::RB];
-  __shared__ __attribute__((aligned(16))) char Q1[T * L::RB];
-  __shared__ __attribute__((aligned(16))) char G0[T * L::RB];  // dO
-  __shared__ __attribute__((aligned(16))) char G1[T * L::RB];
-  __shared__ __attribute__((aligned(16))) float S0[3 * T];  // lse2, delta, document ids
-  __shared__ __attribute__((aligned(16))) float S1[3 * T];
-  __shared__ __attribute__((aligned(16))) char KL[K_IN_LDS ? OWN * L::RB : 16];
+  char *const Q0 = buf.A0, *const Q1 = buf.A1, *const G0 = buf.B0, *const G1 = buf.B1;
+  float *const S0 = buf.S0, *const S1 = buf.S1;
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Sq = a.Sq, Sk = a.Sk;
   const int BHk = a.B * a.Hk;
   // key tile 0 sees the most queries under a causal mask: first
-  const int kt = blockIdx.x / BHk, bk = blockIdx.x % BHk, b = bk / a.Hk, hk = bk % a.Hk;
+  const int kt = item / BHk / a.parts, part = item / BHk % a.parts, bk = item % BHk,
+            b = bk / a.Hk, hk = bk % a.Hk;
   const int k0 = kt * OWN, kw = k0 + 32 * wave, krow = kw + l32;
   const bool wave_valid = kw < Sk;
   const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
@@ -94,7 +142,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
   }
   if (kdoc < 0) qfirst = 0x7fffffff;
 
-  char* const kl = KL + (K_IN_LDS ? wave * 32 * L::RB : 0);
+  char* const kl = buf.own + (K_IN_LDS ? wave * 32 * L::RB : 0);
   u32x4 kf[L::KS], vn[L::KS];
   load_own<E, D>(a.k, b, hk, krow, krow < Sk, a.dch, g, kf);
   load_own<E, D>(a.v, b, hk, krow, krow < Sk, a.dch, g, vn);
@@ -124,26 +172,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
       full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
       pad = w.pad;
     }
-    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
   };
   const int nqt = (Sq + T - 1) / T;
-  // the group's query heads one after another
-  int h = hk * a.G;
-  const int hend = h + a.G;
-  TileScan scan;
-  scan.n = nqt;
-  auto next = [&](int& head) __attribute__((always_inline)) {
-    int t = scan.next(lane, look);
-    while (t < 0 && head + 1 < hend) {
-      ++head;
-      scan = TileScan();
-      scan.n = nqt;
-      t = scan.next(lane, look);
-      if (t < 0) head = hend - 1;  // no tile for one head: none for any
-    }
-    return t;
-  };
-
   Stage<E, D, T> qsrc, gsrc;
   qsrc.init(a.q, b, 0, a.dch, lane, wave);
   gsrc.init(a.dout, b, 0, a.dch, lane, wave);
@@ -173,10 +204,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) dk[i] = dv[i] = f32x16{};
 
-  int cur = next(h);
-  float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-  if (cur >= 0) fetch(cur, h, Q0, G0, S0);
-  __syncthreads();
+  float slope2 = 0.f;
   auto step = [&](int cur, int nxt, int hnext, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
     const char* qt = I ? Q1 : Q0;
@@ -222,11 +250,13 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
         }
         if (!full) {
           const int base = q0 + 32 * qb + 4 * g;
-          const int lo = qfirst == 0x7fffffff ? qfirst : qfirst - a.off - base, hi = Sq - base;
+          // visible: lo <= n < hi, as one unsigned comparison
+          const int lo = qfirst == 0x7fffffff ? 64 : max(qfirst - a.off - base, 0);
+          const uint32_t span = max(Sq - base - lo, 0);
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int n = 8 * (r >> 2) + (r & 3);
-            if (n < lo || n >= hi) s[r] = dp[r] = 0.f;
+            if ((uint32_t)(n - lo) >= span) s[r] = dp[r] = 0.f;
           }
           if (docs) {
 #pragma unroll
@@ -256,18 +286,33 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
     }
     __syncthreads();
   };
-  while (cur >= 0) {
-    int nxt = next(h);
-    step(cur, nxt, h, std::integral_constant<int, 0>{});
-    if (BIAS) slope2 = a.slopes[h] * kLog2e;
-    if ((cur = nxt) < 0) break;
-    nxt = next(h);
-    step(cur, nxt, h, std::integral_constant<int, 1>{});
-    if (BIAS) slope2 = a.slopes[h] * kLog2e;
-    cur = nxt;
+  // the group's query heads one after another
+  for (int first = 0; first < nqt; first += kListed) {
+    TileWalk walk = tile_walk(buf.list, first, nqt, part, a.parts, hk * a.G, a.G, look);
+    int cur = walk.entry();
+    if (cur >= 0) fetch(cur, walk.head, Q0, G0, S0);
+    __syncthreads();
+    while (cur >= 0) {
+      if (BIAS) slope2 = a.slopes[walk.head] * kLog2e;
+      walk.step(walk.parts);
+      int nxt = walk.entry();
+      step(cur, nxt, walk.head, std::integral_constant<int, 0>{});
+      if ((cur = nxt) < 0) break;
+      if (BIAS) slope2 = a.slopes[walk.head] * kLog2e;
+      walk.step(walk.parts);
+      nxt = walk.entry();
+      step(cur, nxt, walk.head, std::integral_constant<int, 1>{});
+      cur = nxt;
+    }
   }
 
   if (!wave_valid) return;
+  if (a.parts > 1) {
+    const int64_t at = 2 * (((int64_t)kt * BHk + bk) * a.parts + part);
+    part_store<L::DB>(dv, part_at<L::DB>(a.part, at, wave), lane);
+    part_store<L::DB>(dk, part_at<L::DB>(a.part, at + 1, wave), lane);
+    return;
+  }
   // idle now: the wave's K rows, or one of the tile buffers
   char* stage = K_IN_LDS ? kl : wave == 0 ? Q0 : wave == 1 ? Q1 : wave == 2 ? G0 : G1;
   const int nrows = min(32, Sk - kw);
@@ -283,23 +328,19 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dkdv_kernel(
 // dQ
 // ---------------------------------------------------------------------------
 template <typename E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SAttnArgs a) {
+__device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buffers& buf) {
   using L = Lay<E, D>;
   constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
-  __shared__ __attribute__((aligned(16))) char K0[T * L::RB];
-  __shared__ __attribute__((aligned(16))) char K1[T * L::RB];
-  __shared__ __attribute__((aligned(16))) char V0[T * L::RB];
-  __shared__ __attribute__((aligned(16))) char V1[T * L::RB];
-  __shared__ __attribute__((aligned(16))) int I0[T];
-  __shared__ __attribute__((aligned(16))) int I1[T];
+  char *const K0 = buf.A0, *const K1 = buf.A1, *const V0 = buf.B0, *const V1 = buf.B1;
+  int *const I0 = (int*)buf.S0, *const I1 = (int*)buf.S1;
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int Sq = a.Sq, Sk = a.Sk;
   const int BH = a.B * a.H, BHk = a.B * a.Hk;
   const int nqt = (Sq + OWN - 1) / OWN;
-  const int qt = nqt - 1 - blockIdx.x / BH;
-  const int n = blockIdx.x % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
+  const int qt = nqt - 1 - item / BH / a.qparts, part = item / BH % a.qparts;
+  const int n = item % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
   const int h = hk * a.G + n / BHk;
   const int q0 = qt * OWN, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
   const bool wave_valid = qw < Sq;
@@ -325,9 +366,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SA
   DocRange own = {0, 0, false};
   if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + 63) / 64);
-  TileScan scan;
-  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk;
-  scan.n = (kend + T - 1) / T;
+  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + T - 1) / T;
   auto look = [&](int t) __attribute__((always_inline)) {
     const int k0 = t * T;
     bool live = !a.causal || k0 <= pmax || k0 < prefix;
@@ -339,7 +378,7 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SA
       full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
       pad = w.pad;
     }
-    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
   };
 
   Stage<E, D, T> ksrc, vsrc;
@@ -363,11 +402,6 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SA
   f32x16 acc[L::DB];
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
-  int cur = scan.next(lane, look);
-  if (cur >= 0) {
-    fetch(cur, K0, V0, I0);
-    __syncthreads();
-  }
   auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
     const char* kt = I ? K1 : K0;
@@ -425,30 +459,110 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_dq_kernel(SA
     }
     __syncthreads();
   };
-  while (cur >= 0) {
-    int nxt = scan.next(lane, look);
-    step(cur, nxt, std::integral_constant<int, 0>{});
-    if ((cur = nxt) < 0) break;
-    nxt = scan.next(lane, look);
-    step(cur, nxt, std::integral_constant<int, 1>{});
-    cur = nxt;
+  for (int first = 0; first < ntiles; first += kListed) {
+    TileWalk walk = tile_walk(buf.list, first, ntiles, part, a.qparts, 0, 1, look);
+    int cur = walk.entry();
+    if (cur >= 0) fetch(cur, K0, V0, I0);
+    __syncthreads();
+    while (cur >= 0) {
+      walk.step(walk.parts);
+      int nxt = walk.entry();
+      step(cur, nxt, std::integral_constant<int, 0>{});
+      if ((cur = nxt) < 0) break;
+      walk.step(walk.parts);
+      nxt = walk.entry();
+      step(cur, nxt, std::integral_constant<int, 1>{});
+      cur = nxt;
+    }
   }
 
   if (!wave_valid) return;
+  if (a.qparts > 1) {
+    const int64_t at = ((int64_t)qt * BH + b * a.H + h) * a.qparts + part;
+    part_store<L::DB>(acc, part_at<L::DB>(a.qpart, at, wave), lane);
+    return;
+  }
   char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
   store_rows<E, D>(acc, a.scale, stage,
                    (char*)a.dq.ptr + (b * a.dq.sb + h * a.dq.sh + qw * a.dq.ss) * L::ESZ,
                    a.dq.ss * L::ESZ, a.dch, min(32, Sq - qw));
 }
 
+// Both kinds in one launch, so that the short items of one fill the gaps that the
+// long ones of the other leave.  Runs of 64 workgroups (whole rounds over the XCDs)
+// belong to one kind, spread evenly; each kind's own order is longest first.
+template <typename E, int D, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_bwd_kernel(SAttnArgs a, int n0,
+                                                                               int n1) {
+  using L = Lay<E, D>;
+  constexpr int T = kTile<E, D>;
+  __shared__ __attribute__((aligned(16))) char A0[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char A1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char B0[T * L::RB];
+  __shared__ __attribute__((aligned(16))) char B1[T * L::RB];
+  __shared__ __attribute__((aligned(16))) float S0[3 * T];
+  __shared__ __attribute__((aligned(16))) float S1[3 * T];
+  __shared__ __attribute__((aligned(16))) char own[L::RB > 128 ? 128 * L::RB : 16];
+  __shared__ int list[kListed];
+  const Buffers buf = {A0, A1, B0, B1, S0, S1, own, list};
+  const int64_t r0 = (n0 + 63) / 64, r = r0 + (n1 + 63) / 64, t = blockIdx.x / 64;
+  const int before = (int)(t * r0 / r);
+  const bool dkdv = (t + 1) * r0 / r > before;
+  const int item = (dkdv ? before : (int)t - before) * 64 + blockIdx.x % 64;
+  if (item >= (dkdv ? n0 : n1)) return;
+  if (dkdv)
+    dkdv_item<E, D, CAP, BIAS>(a, item, buf);
+  else
+    dq_item<E, D, CAP, BIAS>(a, item, buf);
+}
+
+// The sums of split items.  Workgroups [0, n0): dV and dK of the key tiles, two
+// each; then dQ of the query tiles.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void sattn_sum_kernel(SAttnArgs a, int n0) {
+  using L = Lay<E, D>;
+  __shared__ __attribute__((aligned(16))) char stage[4][32 * L::RB];
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool query = (int)blockIdx.x >= n0;
+  const int which = query ? blockIdx.x - n0 : blockIdx.x >> 1, second = query ? 0 : blockIdx.x & 1;
+  const int heads = query ? a.H : a.Hk, n = a.B * heads, tile = which / n, bh = which % n;
+  const int rows = query ? a.Sq : a.Sk, row = 128 * tile + 32 * wave;
+  if (row >= rows) return;
+  f32x16 acc[L::DB];
+#pragma unroll
+  for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  if (query) {
+    for (int i = 0; i < a.qparts; ++i)
+      part_add<L::DB>(acc, part_at<L::DB>(a.qpart, (int64_t)which * a.qparts + i, wave), lane, 1.f);
+  } else {
+    for (int i = 0; i < a.parts; ++i)
+      part_add<L::DB>(acc, part_at<L::DB>(a.part, 2 * ((int64_t)which * a.parts + i) + second, wave),
+                      lane, 1.f);
+  }
+  const TensorArg& t = query ? a.dq : second ? a.dk : a.dv;
+  store_rows<E, D>(acc, query || second ? a.scale : 1.f, stage[wave],
+                   (char*)t.ptr + (bh / heads * t.sb + bh % heads * t.sh + row * t.ss) * L::ESZ,
+                   t.ss * L::ESZ, a.dch, min(32, rows - row));
+}
+
 template <typename E, int D, bool CAP, bool BIAS>
 hipError_t launch_cb(const SAttnArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((sattn_dkdv_kernel<E, D, CAP, BIAS>), dim3((a.Sk + 127) / 128 * a.B * a.Hk),
-                     dim3(256), 0, st, a);
+  const int kitems = (a.Sk + 127) / 128 * a.B * a.Hk, qitems = (a.Sq + 127) / 128 * a.B * a.H;
+  const int n0 = kitems * a.parts, n1 = qitems * a.qparts;
+  hipLaunchKernelGGL((sattn_bwd_kernel<E, D, CAP, BIAS>), dim3(((n0 + 63) / 64 + (n1 + 63) / 64) * 64),
+                     dim3(256), 0, st, a, n0, n1);
   const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((sattn_dq_kernel<E, D, CAP, BIAS>), dim3((a.Sq + 127) / 128 * a.B * a.H),
-                     dim3(256), 0, st, a);
+  const int s0 = a.parts > 1 ? 2 * kitems : 0, s1 = a.qparts > 1 ? qitems : 0;
+  if (e != hipSuccess || s0 + s1 == 0) return e;
+  hipLaunchKernelGGL((sattn_sum_kernel<E, D>), dim3(s0 + s1), dim3(256), 0, st, a, s0);
+  return hipGetLastError();
+}
+
+template <typename E>
+hipError_t launch_delta(const SAttnArgs& a, hipStream_t st) {
+  const uint32_t rows = (uint32_t)a.B * a.H * a.Sq;
+  hipLaunchKernelGGL((sattn_delta_kernel<E>), dim3((rows + 31) / 32), dim3(256), 0, st, a, rows);
   return hipGetLastError();
 }
 
@@ -462,10 +576,36 @@ hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
 
 template <typename E>
 hipError_t launch_e(const SAttnArgs& a, bool cap, hipStream_t st) {
+  const hipError_t e = launch_delta<E>(a, st);
+  if (e != hipSuccess) return e;
   return a.D <= 64 ? launch_d<E, 64>(a, cap, st) : launch_d<E, 128>(a, cap, st);
 }
 
+// Parts of items of `steps` streamed tiles each, when there are n of them: a chain as
+// long as the launch has room for, at least four tiles to a part.
+int parts_of(int64_t n, int64_t steps) {
+  const int64_t most = (steps + 3) / 4, want = 1024 / n;
+  return (int)(want < 2 ? 1 : want < most ? want : most);
+}
+
 }  // namespace
+
+void sattn_bwd_split(SAttnArgs& a, float* ws, int64_t* elems) {
+  const int64_t kitems = (int64_t)((a.Sk + 127) / 128) * a.B * a.Hk;
+  const int64_t qitems = (int64_t)((a.Sq + 127) / 128) * a.B * a.H;
+  const int64_t per = 128 * (a.D <= 64 ? 64 : 128);
+  a.parts = parts_of(kitems, (int64_t)(a.Sq + 63) / 64 * a.G);
+  a.qparts = parts_of(qitems, (a.Sk + 63) / 64);
+  // delta and lse2, then the parts, 16-byte aligned
+  const int64_t rows = ((int64_t)a.B * a.H * a.Sq + 3) / 4 * 4;
+  const int64_t p0 = a.parts > 1 ? 2 * kitems * a.parts * per : 0;
+  const int64_t p1 = a.qparts > 1 ? qitems * a.qparts * per : 0;
+  if (elems) *elems = 2 * rows + p0 + p1;
+  a.delta = ws;
+  a.lse2 = ws + rows;
+  a.part = ws + 2 * rows;
+  a.qpart = a.part + p0;
+}
 
 hipError_t launch_sattn_bwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st) {
   if (dtype == 0) return launch_e<F32>(a, cap, st);

@@ -267,6 +267,12 @@ struct SAttnArgs {
   int causal;
   float scale;
   ScoreConst sc;
+  // Sums split over several workgroups ("parts"), joined by a second launch: O of a
+  // query tile (forward), dK / dV of a key tile and dQ of a query tile (backward).
+  int parts, qparts;     // forward: parts; backward: parts of dK / dV, of dQ
+  float *part, *qpart;   // accumulators as they lie, see part_at
+  float* ml;             // forward: reference and sum of each part's rows
+  void* olo;             // forward: O - round(O), strides of o, or null
 };
 
 // One new token of each sequence over its cache (decode.hip).
@@ -311,36 +317,85 @@ __device__ __forceinline__ DocRange doc_range(const int* ids, int row0, int n, i
   return r;
 }
 
-// The streamed tiles a workgroup has to visit, in order, found 64 at a time: lane
-// t looks at tile base + t, ballots keep the answers in scalar registers.  A
-// tile comes back as its index with kFull (every pair visible: no mask) and
-// kPad (rows of negative document id in it); -1 at the end.
+// The streamed tiles a workgroup has to visit, in order: a list in LDS, built 64
+// tiles at a time (lane t looks at one tile, a ballot gives the live ones their
+// places), at most kListed tiles of the sequence in one list.  An entry is a tile's
+// index with kFull (every pair visible: no mask) and kPad (rows of negative document
+// id in it).  The walk over it, `heads` times for dK / dV, takes the entries part,
+// part + parts, ...: equal shares whatever the mask.
 constexpr int kFull = 1 << 30, kPad = 1 << 29, kTileIndex = kPad - 1;
+constexpr int kListed = 512;
 
-struct TileScan {
-  uint64_t live = 0, full = 0, pad = 0;
-  int base = -64, n;  // n: tiles
-  template <typename F>
-  __device__ __forceinline__ int next(int lane, F look) {
-    while (live == 0) {
-      base += 64;
-      if (base >= n) return -1;
-      const int f = base + lane < n ? look(base + lane) : 0;  // bit 0 live, 1 full, 2 pad
-      live = __ballot(f & 1);
-      full = __ballot(f & 2);
-      pad = __ballot(f & 4);
+struct TileWalk {
+  const int* list;
+  int count, at, parts, head, hend;
+  __device__ __forceinline__ int entry() const {  // -1 behind the last
+    return head < hend ? __builtin_amdgcn_readfirstlane(list[at]) : -1;
+  }
+  __device__ __forceinline__ void step(int n) {
+    at += n;
+    while (at >= count && head < hend) {
+      at -= count;
+      ++head;
     }
-    const int i = __builtin_ctzll(live);
-    live &= live - 1;
-    return (base + i) | ((full >> i) & 1 ? kFull : 0) | ((pad >> i) & 1 ? kPad : 0);
   }
 };
+
+// Tiles [first, first + kListed) of n; `look` says of one: bit 0 live, kFull, kPad.
+// Ends with a barrier.
+template <typename F>
+__device__ __forceinline__ TileWalk tile_walk(int* list, int first, int n, int part, int parts,
+                                              int head, int heads, F look) {
+  const int lane = threadIdx.x & 63, end = min(n, first + kListed);
+  int count = 0;
+  for (int t0 = first; t0 < end; t0 += 64) {
+    const int f = t0 + lane < end ? look(t0 + lane) : 0;
+    const uint64_t live = __ballot(f & 1);
+    if ((f & 1) && threadIdx.x < 64)
+      list[count + __popcll(live & ((1ull << lane) - 1))] = (t0 + lane) | (f & (kFull | kPad));
+    count += __popcll(live);
+  }
+  __syncthreads();
+  TileWalk w = {list, count, 0, parts, count ? head : head + heads, head + heads};
+  if (count) w.step(part);
+  return w;
+}
+
+// A part's accumulators (32 rows of a wave, DB column blocks) in the workspace, as
+// they lie in the registers: whole 1 KB stores and loads.  `index`: which tile,
+// tensor and part.
+template <int DB>
+__device__ __forceinline__ f32x4* part_at(float* part, int64_t index, int wave) {
+  return (f32x4*)(part + (index * 4 + wave) * (DB * 1024));
+}
+template <int DB>
+__device__ __forceinline__ void part_store(const f32x16 (&acc)[DB], f32x4* p, int lane) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj)
+      p[(4 * db + jj) * 64 + lane] = f32x4{acc[db][4 * jj], acc[db][4 * jj + 1],
+                                           acc[db][4 * jj + 2], acc[db][4 * jj + 3]};
+}
+// acc += w * the part
+template <int DB>
+__device__ __forceinline__ void part_add(f32x16 (&acc)[DB], const f32x4* p, int lane, float w) {
+#pragma unroll
+  for (int db = 0; db < DB; ++db)
+#pragma unroll
+    for (int jj = 0; jj < 4; ++jj) {
+      const f32x4 x = p[(4 * db + jj) * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[db][4 * jj + i] = __builtin_fmaf(x[i], w, acc[db][4 * jj + i]);
+    }
+}
 
 // Writes one wave's 32 x D block, held transposed in 32x32 accumulators, times a
 // per-lane factor, rounded to E: staged through the wave's own LDS region (32
 // rows) so that each lane stores 16 contiguous bytes.  Chunks at or past dch and
 // rows at or past nrows are not stored.
-template <typename E, int D>
+// LO (16-bit types): what the rounding to E leaves, rounded to E, instead.
+template <typename E, int D, bool LO = false>
 __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float sc, char* lds,
                                            char* out, int64_t row_bytes, int dch, int nrows) {
   using L = Lay<E, D>;
@@ -356,8 +411,11 @@ __device__ __forceinline__ void store_rows(const f32x16 (&acc)[D / 32], float sc
         *(f32x4*)(lds + l32 * L::RB + ((ch ^ (l32 & 7)) << 4)) = f32x4{a, b, c, d};
       } else {
         const int ch = 4 * db + jj;
-        *(u32x2*)(lds + l32 * L::RB + ((ch ^ (l32 & 7)) << 4) + 8 * g) =
-            Elem<E>::pack4(a, b, c, d);
+        u32x2 w = Elem<E>::pack4(a, b, c, d);
+        if constexpr (LO)
+          w = Elem<E>::pack4(a - E::to_f32(w[0] & 0xffff), b - E::to_f32(w[0] >> 16),
+                             c - E::to_f32(w[1] & 0xffff), d - E::to_f32(w[1] >> 16));
+        *(u32x2*)(lds + l32 * L::RB + ((ch ^ (l32 & 7)) << 4) + 8 * g) = w;
       }
     }
 #pragma unroll

@@ -10,12 +10,14 @@
 // keep a query per lane, so the softmax's statistics are per-lane scalars and P
 // feeds the second product from the accumulators; 64-key tiles of K and V come
 // in by direct global -> LDS loads, double buffered, one barrier per tile.
-//   * Which key tiles a workgroup visits is found 64 at a time by ballot
-//     (TileScan) from positions, the prefix and the 64-key ranges of document
+//   * Which key tiles a workgroup visits is listed beforehand
+//     (tile_walk) from positions, the prefix and the 64-key ranges of document
 //     ids: tiles without a visible pair cost nothing, tiles where every pair is
 //     visible run without mask code.
 //   * Query heads that share a key head go to the same XCD (workgroups are dealt
 //     round robin over the 8 XCDs), so that its L2 reads K and V once for all.
+//   * Small grids split a query tile's keys into parts (fwd_parts), joined by a second
+//     launch.
 //   * Head dims below 64 and between 64 and 128 run in the next layout with zero
 //     chunks.
 #include <type_traits>
@@ -40,6 +42,23 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* docs, DocTile
   if (lane == 0) out[i] = DocTile{r.lo, r.hi, r.pad, 0};
 }
 
+// A wave's O (normalised) and lse.  A row without a visible key: O = 0, lse = -inf.
+template <typename E, int D>
+__device__ __forceinline__ void finish_rows(const SAttnArgs& a, int b, int h, int qw,
+                                            const f32x16 (&acc)[D / 32], float m, float l,
+                                            char* stage) {
+  using L = Lay<E, D>;
+  const int lane = threadIdx.x & 63, qrow = qw + (lane & 31), nrows = min(32, a.Sq - qw);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = (b * a.o.sb + h * a.o.sh + qw * a.o.ss) * L::ESZ, row = a.o.ss * L::ESZ;
+  store_rows<E, D>(acc, inv, stage, (char*)a.o.ptr + at, row, a.dch, nrows);
+  if constexpr (L::ESZ == 2)
+    if (a.olo) store_rows<E, D, true>(acc, inv, stage, (char*)a.olo + at, row, a.dch, nrows);
+  if (lane < 32 && qrow < a.Sq)
+    a.lse[((int64_t)b * a.H + h) * a.Sq + qrow] =
+        l == 0.f ? -INFINITY : (m + fast_log2(l)) * kLn2;
+}
+
 constexpr float kSlack = 8.f;  // log2 units a score may exceed the running reference by
 
 template <typename E, int D, bool CAP, bool BIAS>
@@ -52,6 +71,7 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
   __shared__ __attribute__((aligned(16))) char V1[BK * L::RB];
   __shared__ __attribute__((aligned(16))) int I0[BK];  // document ids of the keys
   __shared__ __attribute__((aligned(16))) int I1[BK];
+  __shared__ int list[kListed];
 
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, g = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -61,7 +81,7 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
   // heads run fastest, then the query heads of a group
   const int BH = a.B * a.H, BHk = a.B * a.Hk;
   const int nqt = (Sq + BQ - 1) / BQ;
-  const int qt = nqt - 1 - blockIdx.x / BH;
+  const int part = blockIdx.x / BH % a.parts, qt = nqt - 1 - blockIdx.x / BH / a.parts;
   const int n = blockIdx.x % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
   const int h = hk * a.G + n / BHk;
 
@@ -90,9 +110,7 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
   DocRange own = {0, 0, false};
   if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + BK - 1) / BK);
-  TileScan scan;
-  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk;
-  scan.n = (kend + BK - 1) / BK;
+  const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + BK - 1) / BK;
   auto look = [&](int t) __attribute__((always_inline)) {
     const int k0 = t * BK;
     bool live = !a.causal || k0 <= pmax || k0 < prefix;
@@ -104,7 +122,7 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
       full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
       pad = w.pad;
     }
-    return (live ? 1 : 0) | (full ? 2 : 0) | (pad ? 4 : 0);
+    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
   };
 
   Stage<E, D, BK> ksrc, vsrc;
@@ -133,11 +151,6 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
   // factor that takes a score to log2 units
   const float c = CAP || BIAS ? 1.f : a.sc.c;
 
-  int cur = scan.next(lane, look);
-  if (cur >= 0) {
-    fetch(cur, K0, V0, I0);
-    __syncthreads();
-  }
   auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
     const char* kt = I ? K1 : K0;
@@ -203,13 +216,13 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] = fast_exp2(__builtin_fmaf(s[kb][r], c, -ref));
-#pragma unroll
-        for (int ng = 0; ng < L::NG; ++ng) {
-          p[kb][ng] = Elem<E>::operand(s[kb], ng);
-          // P as rounded for the product, so that O / l normalises what it applied
-          ps[ng & 1] = Elem<E>::sum(p[kb][ng], ps[ng & 1]);
+        for (int r = 0; r < 16; ++r) {
+          s[kb][r] = fast_exp2(__builtin_fmaf(s[kb][r], c, -ref));
+          // the sum before P is rounded for the product: lse is an fp32 result
+          ps[r & 1] += s[kb][r];
         }
+#pragma unroll
+        for (int ng = 0; ng < L::NG; ++ng) p[kb][ng] = Elem<E>::operand(s[kb], ng);
       }
       l_run += ps[0] + ps[1];
 #pragma unroll
@@ -222,30 +235,80 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
     }
     __syncthreads();
   };
-  while (cur >= 0) {
-    int nxt = scan.next(lane, look);
-    step(cur, nxt, std::integral_constant<int, 0>{});
-    if ((cur = nxt) < 0) break;
-    nxt = scan.next(lane, look);
-    step(cur, nxt, std::integral_constant<int, 1>{});
-    cur = nxt;
+  for (int first = 0; first < ntiles; first += kListed) {
+    TileWalk walk = tile_walk(list, first, ntiles, part, a.parts, 0, 1, look);
+    int cur = walk.entry();
+    if (cur >= 0) fetch(cur, K0, V0, I0);
+    __syncthreads();
+    while (cur >= 0) {
+      walk.step(walk.parts);
+      int nxt = walk.entry();
+      step(cur, nxt, std::integral_constant<int, 0>{});
+      if ((cur = nxt) < 0) break;
+      walk.step(walk.parts);
+      nxt = walk.entry();
+      step(cur, nxt, std::integral_constant<int, 1>{});
+      cur = nxt;
+    }
   }
 
   if (!wave_valid) return;
-  // a row without a visible key: O = 0, lse = -inf
   const float l = sum_halves(l_run);
   char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
-  store_rows<E, D>(acc, l == 0.f ? 0.f : 1.f / l, stage,
-                   (char*)a.o.ptr + (b * a.o.sb + h * a.o.sh + qw * a.o.ss) * L::ESZ,
-                   a.o.ss * L::ESZ, a.dch, min(32, Sq - qw));
-  if (g == 0 && qrow < Sq)
-    a.lse[((int64_t)b * a.H + h) * Sq + qrow] =
-        l == 0.f ? -INFINITY : (m_run + fast_log2(l)) * kLn2;
+  if (a.parts > 1) {
+    const int64_t at = ((int64_t)qt * BH + b * a.H + h) * a.parts + part;
+    part_store<L::DB>(acc, part_at<L::DB>(a.part, at, wave), lane);
+    float* ml = a.ml + (at * 4 + wave) * 64;
+    if (g == 0) {
+      ml[l32] = m_run;
+      ml[32 + l32] = l;
+    }
+    return;
+  }
+  finish_rows<E, D>(a, b, h, qw, acc, m_run, l, stage);
+}
+
+// O and lse of query tiles split into parts: each row's parts taken to their common
+// reference and added in order.
+template <typename E, int D>
+__global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a) {
+  using L = Lay<E, D>;
+  __shared__ __attribute__((aligned(16))) char stage[4][32 * L::RB];
+  const int lane = threadIdx.x & 63, l32 = lane & 31;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int BH = a.B * a.H, qt = blockIdx.x / BH, bh = blockIdx.x % BH, qw = qt * 128 + 32 * wave;
+  if (qw >= a.Sq) return;
+  const int64_t at = (int64_t)blockIdx.x * a.parts;
+  float m = -INFINITY;
+  for (int i = 0; i < a.parts; ++i) m = fmaxf(m, a.ml[((at + i) * 4 + wave) * 64 + l32]);
+  const float ref = m == -INFINITY ? 0.f : m;
+  f32x16 acc[L::DB];
+#pragma unroll
+  for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  float l = 0.f;
+  for (int i = 0; i < a.parts; ++i) {
+    const float* ml = a.ml + ((at + i) * 4 + wave) * 64;
+    const float w = fast_exp2(ml[l32] - ref);
+    l = __builtin_fmaf(ml[32 + l32], w, l);
+    part_add<L::DB>(acc, part_at<L::DB>(a.part, at + i, wave), lane, w);
+  }
+  finish_rows<E, D>(a, bh / a.H, bh % a.H, qw, acc, m, l, stage[wave]);
+}
+
+// Parts a query tile's keys are split into.  A workgroup is a serial chain of key
+// tiles, and a launch of few of them leaves the chip empty; a split costs writing
+// and reading the parts' fp32 O once.  Up to one workgroup per CU, no fewer than
+// four key tiles to a part.
+int fwd_parts(const SAttnArgs& a) {
+  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H;
+  const int64_t most = (a.Sk + 255) / 256, want = 512 / n;
+  return (int)(want < 2 ? 1 : want < most ? want : most);
 }
 
 template <typename E, int D>
 hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
-  const dim3 grid((a.Sq + 127) / 128 * a.B * a.H), block(256);
+  const int n = (a.Sq + 127) / 128 * a.B * a.H;
+  const dim3 grid(n * a.parts), block(256);
   if (cap && a.slopes)
     hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, true>), grid, block, 0, st, a);
   else if (cap)
@@ -254,6 +317,9 @@ hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
     hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, true>), grid, block, 0, st, a);
   else
     hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, false>), grid, block, 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  hipLaunchKernelGGL((sattn_join_kernel<E, D>), dim3(n), block, 0, st, a);
   return hipGetLastError();
 }
 
@@ -270,6 +336,18 @@ hipError_t launch_doc_tiles(const int* docs, void* tiles, int B, int Sq, int Sk,
   hipLaunchKernelGGL(doc_tiles_kernel, dim3((uint32_t)((n + 3) / 4)), dim3(256), 0, st, docs,
                      (DocTile*)tiles, B, Sq, Sk, nk, nq);
   return hipGetLastError();
+}
+
+int64_t sattn_fwd_workspace(const SAttnArgs& a) {
+  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H, p = fwd_parts(a);
+  return p == 1 ? 0 : n * p * (128 * (a.D <= 64 ? 64 : 128) + 256);
+}
+
+void sattn_fwd_split(SAttnArgs& a, float* ws) {
+  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H;
+  a.parts = fwd_parts(a);
+  a.part = ws;
+  a.ml = ws + n * a.parts * (128 * (a.D <= 64 ? 64 : 128));
 }
 
 hipError_t launch_sattn_fwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st) {

@@ -52,7 +52,8 @@ using torch::autograd::variable_list;
   X(mi_rmsnorm_add_fwd) X(mi_rmsnorm_add_bwd) X(mi_rmsnorm_add_bwd_acc) X(mi_swiglu_fwd)   \
   X(mi_swiglu_bwd) X(mi_wgrad_suits) X(mi_wgrad_workspace) X(mi_wgrad)                     \
   X(mi_rotary_qk) X(mi_qk_norm_rotary) X(mi_qk_norm_rotary_workspace)                      \
-  X(mi_qk_norm_rotary_bwd) X(mi_sattn_tiles) X(mi_sattn_fwd) X(mi_sattn_bwd_workspace)     \
+  X(mi_qk_norm_rotary_bwd) X(mi_sattn_tiles) X(mi_sattn_fwd_workspace) X(mi_sattn_fwd)      \
+  X(mi_sattn_bwd_workspace)                                                                \
   X(mi_sattn_bwd) X(mi_decode_workspace) X(mi_decode_attn)
 
 struct Bound {
@@ -842,32 +843,37 @@ Mods dense_mods(const Mods& m) {
 }
 
 struct SAttnOut {
-  Tensor o, lse, tiles;
+  Tensor o, lo, lse, tiles;  // lo: what rounding o left (16-bit types, for the backward)
 };
 // q, k, v by rows_ready, m by dense_mods.
-SAttnOut sattn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Mods& m) {
+SAttnOut sattn_fwd(const Tensor& q, const Tensor& k, const Tensor& v, const Mods& m, bool grad) {
   const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1),
                 Sk = k.size(2);
-  SAttnOut r{empty({B, H, Sq, D}, q), empty_f32({B, H, Sq}, q), Tensor()};
+  SAttnOut r{empty({B, H, Sq, D}, q), Tensor(), empty_f32({B, H, Sq}, q), Tensor()};
+  if (grad && code(q) != MI_F32) r.lo = empty({B, H, Sq, D}, q);
   if (m.docs.defined())
     r.tiles = at::empty({lib.mi_sattn_tiles(B, Sq, Sk)}, q.options().dtype(at::kInt));
   const mi_score_mods c = c_mods(m);
+  const int64_t n = lib.mi_sattn_fwd_workspace(dt(q), B, H, Hk, Sq, Sk, D);
+  Tensor ws = n ? empty_f32({n}, q) : Tensor();
   check(lib.mi_sattn_fwd(dt(q), B, H, Hk, Sq, Sk, D, m.scale, &c, q.data_ptr(), Strides(q).s,
                          k.data_ptr(), Strides(k).s, v.data_ptr(), Strides(v).s, r.o.data_ptr(),
-                         Strides(r.o).s, r.lse.data_ptr<float>(),
-                         r.tiles.defined() ? r.tiles.data_ptr<int32_t>() : nullptr, stream(q)),
+                         Strides(r.o).s, r.lo.defined() ? r.lo.data_ptr() : nullptr,
+                         r.lse.data_ptr<float>(),
+                         r.tiles.defined() ? r.tiles.data_ptr<int32_t>() : nullptr,
+                         n ? ws.data_ptr<float>() : nullptr, n, stream(q)),
         "mi_sattn_fwd");
   return r;
 }
 
 struct ScoredAttn : torch::autograd::Function<ScoredAttn> {
   static Tensor forward(AutogradContext* ctx, const Tensor& q_, const Tensor& k_, const Tensor& v_,
-                        const Mods& m_) {
+                        const Mods& m_, bool grad) {
     const c10::DeviceGuard guard(q_.device());
     const Tensor q = rows_ready(q_), k = rows_ready(k_), v = rows_ready(v_);
     const Mods m = dense_mods(m_);
-    const SAttnOut r = sattn_fwd(q, k, v, m);
-    ctx->save_for_backward({q, k, v, r.o, r.lse, r.tiles, m.slopes, m.docs, m.prefix});
+    const SAttnOut r = sattn_fwd(q, k, v, m, grad);
+    ctx->save_for_backward({q, k, v, r.o, r.lo, r.lse, r.tiles, m.slopes, m.docs, m.prefix});
     ctx->saved_data["causal"] = m.causal;
     ctx->saved_data["cap"] = m.cap;
     ctx->saved_data["scale"] = m.scale;
@@ -876,9 +882,10 @@ struct ScoredAttn : torch::autograd::Function<ScoredAttn> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lse = s[4], &tiles = s[5];
+    const Tensor &q = s[0], &k = s[1], &v = s[2], &o = s[3], &lo = s[4], &lse = s[5],
+                 &tiles = s[6];
     const Mods m{ctx->saved_data["causal"].toBool(), ctx->saved_data["cap"].toDouble(),
-                 ctx->saved_data["scale"].toDouble(), s[6], s[7], s[8]};
+                 ctx->saved_data["scale"].toDouble(), s[7], s[8], s[9]};
     check_leaves(ctx, grads[0]);
     const Tensor go = rows_ready(grads[0]);
     const c10::DeviceGuard guard(go.device());
@@ -887,6 +894,7 @@ struct ScoredAttn : torch::autograd::Function<ScoredAttn> {
     const int64_t B = q.size(0), H = q.size(1), Sq = q.size(2), D = q.size(3), Hk = k.size(1),
                   Sk = k.size(2);
     dense("output", o, {B, H, Sq, D}, q.scalar_type(), q);
+    if (lo.defined()) dense("rest of the output", lo, {B, H, Sq, D}, q.scalar_type(), q);
     dense("lse", lse, {B, H, Sq}, at::kFloat, q);
     if (m.slopes.defined()) dense("slopes", m.slopes, {H}, at::kFloat, q);
     if (m.prefix.defined()) dense("prefix_lens", m.prefix, {B}, at::kInt, q);
@@ -901,12 +909,13 @@ struct ScoredAttn : torch::autograd::Function<ScoredAttn> {
     const mi_score_mods c = c_mods(m);
     check(lib.mi_sattn_bwd(dt(q), B, H, Hk, Sq, Sk, D, m.scale, &c, q.data_ptr(), Strides(q).s,
                            k.data_ptr(), Strides(k).s, v.data_ptr(), Strides(v).s, o.data_ptr(),
-                           Strides(o).s, go.data_ptr(), Strides(go).s, lse.data_ptr<float>(),
+                           Strides(o).s, lo.defined() ? lo.data_ptr() : nullptr, go.data_ptr(),
+                           Strides(go).s, lse.data_ptr<float>(),
                            tiles.defined() ? tiles.data_ptr<int32_t>() : nullptr,
                            ws.data_ptr<float>(), n, dq.data_ptr(), Strides(dq).s, dk.data_ptr(),
                            Strides(dk).s, dv.data_ptr(), Strides(dv).s, stream(q)),
           "mi_sattn_bwd");
-    return {dq, dk, dv, Tensor()};
+    return {dq, dk, dv, Tensor(), Tensor()};
   }
 };
 
@@ -1156,7 +1165,9 @@ PyObject* py_scored_attn(PyObject*, Args a, Py_ssize_t n) {
   Tensor q, k, v;
   Mods m;
   PLAIN(sattn_args(a, n, q, k, v, m));
-  return THPVariable_Wrap(released([&] { return ScoredAttn::apply(q, k, v, m); }));
+  const bool grad = at::GradMode::is_enabled() &&
+                    (q.requires_grad() || k.requires_grad() || v.requires_grad());
+  return THPVariable_Wrap(released([&] { return ScoredAttn::apply(q, k, v, m, grad); }));
   END_HANDLE_TH_ERRORS
 }
 
@@ -1168,7 +1179,7 @@ PyObject* py_scored_attn_forward(PyObject*, Args a, Py_ssize_t n) {
   const SAttnOut r = released([&] {
     const c10::DeviceGuard guard(q.device());
     const at::NoGradGuard no_grad;
-    return sattn_fwd(rows_ready(q), rows_ready(k), rows_ready(v), dense_mods(m));
+    return sattn_fwd(rows_ready(q), rows_ready(k), rows_ready(v), dense_mods(m), false);
   });
   return pair(r.o, r.lse);
   END_HANDLE_TH_ERRORS

@@ -92,33 +92,35 @@ def _scale(q, scale):
     return 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
 
 
-def _forward(q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale):
+def _forward(q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale, grad=False):
     _check(q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale)
     q, k, v = (_lib.rows_ready(t) for t in (q, k, v))
     mods = (bool(causal), softcap, _dense(slopes), _dense(document_ids), _dense(prefix_lens))
     with torch.cuda.device(q.device):
-        return (q, k, v), mods, _lib.sattn_fwd(q, k, v, mods, scale)
+        return (q, k, v), mods, _lib.sattn_fwd(q, k, v, mods, scale, grad)
 
 
 class ScoredAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale):
-        qkv, mods, (o, lse, tiles) = _forward(q, k, v, causal, softcap, slopes, document_ids,
-                                              prefix_lens, scale)
-        ctx.save_for_backward(*qkv, o, lse, tiles, *mods[2:])
+        qkv, mods, (o, o_lo, lse, tiles) = _forward(q, k, v, causal, softcap, slopes, document_ids,
+                                                    prefix_lens, scale, any(ctx.needs_input_grad))
+        ctx.save_for_backward(*qkv, o, o_lo, lse, tiles, *mods[2:])
         ctx.meta = mods[0], mods[1], scale
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, lse, tiles, slopes, docs, prefix = ctx.saved_tensors
+        q, k, v, o, o_lo, lse, tiles, slopes, docs, prefix = ctx.saved_tensors
         causal, softcap, scale = ctx.meta
         do = _lib.rows_ready(do.to(q.dtype))
         # what was saved may come back through a saved-tensor hook as something else
         _check(q, k, v, causal, softcap, slopes, docs, prefix, scale)
         if do.shape != q.shape or o.shape != q.shape or o.dtype != q.dtype \
                 or lse.shape != q.shape[:3] or lse.dtype != torch.float32 \
-                or not all(t.is_contiguous() for t in (o, lse)):
+                or not all(t.is_contiguous() for t in (o, lse)) \
+                or (o_lo is not None and (o_lo.shape != o.shape or o_lo.dtype != o.dtype
+                                          or not o_lo.is_contiguous())):
             raise ValueError("the gradient and the saved tensors do not fit each other")
         if docs is not None and (tiles.dtype != torch.int32 or not tiles.is_contiguous()
                                  or tiles.numel() != _lib.sattn_tiles(q, k)):
@@ -126,7 +128,7 @@ class ScoredAttn(torch.autograd.Function):
         q, k, v = (_lib.rows_ready(t) for t in (q, k, v))
         slopes, docs, prefix = _dense(slopes), _dense(docs), _dense(prefix)
         with torch.cuda.device(q.device):
-            grads = _lib.sattn_bwd(q, k, v, o, do, lse, tiles,
+            grads = _lib.sattn_bwd(q, k, v, o, o_lo, do, lse, tiles,
                                    (causal, softcap, slopes, docs, prefix), scale)
         return (*grads, None, None, None, None, None, None)
 
@@ -151,8 +153,9 @@ def scored_attn_forward(q, k, v, causal: bool = True, softcap=None, slopes=None,
     if out is not None:
         return out
     with torch.no_grad():
-        return _forward(q, k, v, causal, softcap, slopes, document_ids, prefix_lens,
-                        _scale(q, softmax_scale))[2][:2]
+        o, _, lse, _ = _forward(q, k, v, causal, softcap, slopes, document_ids, prefix_lens,
+                                _scale(q, softmax_scale))[2]
+        return o, lse
 
 
 def decode_attn(q, k, v, lengths=None, softcap=None, slopes=None, softmax_scale=None):

@@ -566,25 +566,32 @@ typedef struct mi_score_mods {
  * document_ids are given and the backward reads. */
 int64_t mi_sattn_tiles(int B, int Sq, int Sk);
 
+/* Floats of workspace that mi_sattn_fwd needs (16-byte aligned; 0: none, NULL will
+ * do).  o_lo (as o, same strides, 16-bit types only; may be NULL): what rounding O
+ * to its type left, for the backward. */
+int64_t mi_sattn_fwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D);
+
 mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
                        const mi_score_mods* mods,
                        const void* q, const int64_t q_strides[4],
                        const void* k, const int64_t k_strides[4],
                        const void* v, const int64_t v_strides[4],
-                       void* o, const int64_t o_strides[4], float* lse /* [B, H, Sq] */,
-                       int32_t* tiles, void* stream);
+                       void* o, const int64_t o_strides[4], void* o_lo,
+                       float* lse /* [B, H, Sq] */, int32_t* tiles,
+                       float* workspace, int64_t workspace_elems, void* stream);
 
 /* Floats of workspace that mi_sattn_bwd needs (16-byte aligned). */
 int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D);
 
 /* dQ [B, H, Sq, D], dK and dV [B, Hk, Sk, D] (summed over the query heads of each
- * key head); no atomics: the same bits every time. */
+ * key head); no atomics: the same bits every time.  o_lo: the forward's, or NULL
+ * (then delta = rowsum(dO * O) takes over O's rounding). */
 mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,
                        const mi_score_mods* mods,
                        const void* q, const int64_t q_strides[4],
                        const void* k, const int64_t k_strides[4],
                        const void* v, const int64_t v_strides[4],
-                       const void* o, const int64_t o_strides[4],
+                       const void* o, const int64_t o_strides[4], const void* o_lo,
                        const void* dout, const int64_t dout_strides[4],
                        const float* lse, const int32_t* tiles,
                        float* workspace, int64_t workspace_elems,

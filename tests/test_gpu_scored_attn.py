@@ -143,17 +143,20 @@ def test_long_keys(gpu, dtype):
     run(dict(size=(1, 1, 1, 200, 4500, 128), causal=False, cap=30.0), dtype, gpu)
 
 
-def test_many_documents_skip_everything_between(gpu):
-    """Long packed sequence: a document gives what it gives alone, bit for bit as far
-    as the tiles it meets are the same ones."""
+def test_many_documents_as_if_alone(gpu):
+    """A long packed sequence: each document gives what it gives alone, within the
+    bounds of both (the two calls may split their sums differently)."""
     from gpt_from_scratch_amd import scored_attn_forward
     D, S = 64, 2048
     q, k, v = (randn((1, 4, S, D), i, torch.bfloat16, gpu) for i in range(3))
     ids = (torch.arange(S, dtype=torch.int32, device=gpu) // 256)[None]
     o, lse = scored_attn_forward(q, k, v, document_ids=ids)
     for a in range(0, S, 256):
-        oa, la = scored_attn_forward(*(t[:, :, a:a + 256] for t in (q, k, v)))
-        assert torch.equal(oa, o[:, :, a:a + 256]) and torch.equal(la, lse[:, :, a:a + 256])
+        part = [t[:, :, a:a + 256] for t in (q, k, v)]
+        want = ref.attention(*part)
+        for got in ((o[:, :, a:a + 256], lse[:, :, a:a + 256]), scored_attn_forward(*part)):
+            ref.within("o", got[0], want["o"])
+            ref.within("lse", got[1], want["lse"])
 
 
 @pytest.mark.parametrize("dtype", TYPES)
