@@ -1371,13 +1371,14 @@ mi_status check_workspace(const float* ws, int64_t have, int64_t want) {
   return MI_OK;
 }
 
-mi::ScoreConst score_const(float scale, float softcap) {
+mi::ScoreConst score_const(mi_dtype dtype, float scale, float softcap) {
   mi::ScoreConst c = {};
-  c.c = scale * 1.4426950408889634f;
-  if (softcap > 0.f) {
+  c.f = (float)(1.4426950408889634 * scale);
+  if (softcap > 0.f) {  // in the form sattn_device.h's score_y gives each type
+    c.f = (float)(1.4426950408889634 * softcap * (dtype == MI_F32 ? 1.0 : 2.0));
+    c.b0 = dtype == MI_F32 ? 0.f : (float)(1.4426950408889634 * softcap);
     c.kz = scale / softcap;
     c.k1 = (float)(2.0 * 1.4426950408889634 * scale / softcap);
-    c.capl2 = (float)(1.4426950408889634 * softcap);
   }
   return c;
 }
@@ -1395,7 +1396,7 @@ mi::SAttnArgs sattn_args(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, i
   a.dch = D * elem_size(dtype) / 16;
   a.causal = m.causal ? 1 : 0;
   a.scale = scale;
-  a.sc = score_const(scale, m.softcap);
+  a.sc = score_const(dtype, scale, m.softcap);
   return a;
 }
 
@@ -1527,7 +1528,7 @@ mi_status mi_decode_attn(mi_dtype dtype, int B, int H, int Hk, int S, int D, flo
   a.B = B; a.H = H; a.Hk = Hk; a.G = H / Hk; a.S = S; a.D = D;
   a.dch = D * esz / 16;
   a.splits = mi::decode_splits(dtype, B, H, Hk, S, D);
-  a.sc = score_const(scale, softcap);
+  a.sc = score_const(dtype, scale, softcap);
   a.part = workspace;
   a.ml = workspace + (int64_t)B * H * a.splits * D;
   return launched(mi::launch_decode(dtype, a, softcap > 0.f, (hipStream_t)stream), "decode");

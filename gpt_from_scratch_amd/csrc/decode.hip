@@ -71,7 +71,6 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  const float c = CAP || BIAS ? 1.f : a.sc.c;
   if (t0 < t1) {
     ksrc.load(t0 * TK, len, K0, wave);
     vsrc.load(t0 * TK, len, V0, wave);
@@ -92,13 +91,12 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
 #pragma unroll
       for (int ks = 0; ks < L::KS; ++ks)
         s = Elem<E>::mfma(rd.row(kt, 0, ks), qf[ks], ks == 0 ? f32x16{} : s);
-      if constexpr (CAP || BIAS) {
-        const float d0 = (float)(len - 1 - k0 - 4 * g);
+      const float d0 = (float)(len - 1 - k0 - 4 * g);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float tanh_z;
-          s[r] = score<E, CAP, BIAS>(s[r], d0 - (8 * (r >> 2) + (r & 3)), slope2, a.sc, tanh_z);
-        }
+      for (int r = 0; r < 16; ++r) {
+        s[r] = score_y<E, CAP>(s[r], a.sc) * a.sc.f;
+        // no key is behind the query's position, which is the last
+        if constexpr (BIAS) s[r] = __builtin_fmaf(-slope2, d0 - (8 * (r >> 2) + (r & 3)), s[r]);
       }
       if (k0 + 32 > len) {
         const int rel = len - k0 - 4 * g;
@@ -109,7 +107,7 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
       float mx = vmax(s[0], s[1]);
 #pragma unroll
       for (int r = 2; r < 16; r += 2) mx = vmax(vmax(mx, s[r]), s[r + 1]);
-      mx = max_halves(mx) * c;
+      mx = max_halves(mx);
       if (__any(mx > m_run)) {
         const float m_new = fmaxf(m_run, mx);
         const float alpha = fast_exp2(m_run - (m_new == -INFINITY ? 0.f : m_new));
@@ -120,7 +118,7 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
       }
       const float ref = m_run == -INFINITY ? 0.f : m_run;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -ref));
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(s[r] - ref);
 #pragma unroll
       for (int ng = 0; ng < L::NG; ++ng) {
         const u32x4 p = Elem<E>::operand(s, ng);
@@ -182,12 +180,13 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
   }
 }
 
-// O of one row from its parts: a wave per row, lane d, d + 64.
+// O of one row from its parts: a workgroup per row, its waves a quarter of the parts
+// each, lane d, d + 64 (one wave over 64 parts, a chain of 64 loads, took 35 us).
 template <typename E>
 __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
-  const int lane = threadIdx.x & 63;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (row >= (int64_t)a.B * a.H) return;
+  __shared__ float sum[4][128], weight[64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
   // splits <= 64: a part per lane
   float m = -INFINITY, l = 0.f;
   if (lane < a.splits) {
@@ -201,17 +200,23 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   float lt = l * f;
 #pragma unroll
   for (int x = 32; x; x >>= 1) lt += __shfl_xor(lt, x, 64);
+  if (wave == 0) weight[lane] = f;
+  __syncthreads();
   const float* part = a.part + row * a.splits * a.D;
   float o0 = 0.f, o1 = 0.f;
-  for (int s = 0; s < a.splits; ++s) {
-    const float w = __shfl(f, s, 64);
+#pragma unroll 8
+  for (int s = wave; s < a.splits; s += 4) {
+    const float w = weight[s];
     if (lane < a.D) o0 = __builtin_fmaf(part[s * a.D + lane], w, o0);
     if (lane + 64 < a.D) o1 = __builtin_fmaf(part[s * a.D + lane + 64], w, o1);
   }
-  const float inv = lt == 0.f ? 0.f : 1.f / lt;
-  const int64_t out = row / a.H * a.o_sb + row % a.H * a.o_sh;
-  if (lane < a.D) put<E>(a.o, out + lane, o0 * inv);
-  if (lane + 64 < a.D) put<E>(a.o, out + lane + 64, o1 * inv);
+  sum[wave][lane] = o0;
+  sum[wave][lane + 64] = o1;
+  __syncthreads();
+  const int d = threadIdx.x;
+  if (d >= a.D) return;
+  const float o = (sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]);
+  put<E>(a.o, row / a.H * a.o_sb + row % a.H * a.o_sh + d, lt == 0.f ? 0.f : o / lt);
 }
 
 template <typename E, int D>
@@ -227,8 +232,7 @@ hipError_t launch_d(const DecodeArgs& a, bool cap, hipStream_t st) {
     hipLaunchKernelGGL((decode_kernel<E, D, false, false>), grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((decode_join_kernel<E>), dim3((uint32_t)(((int64_t)a.B * a.H + 3) / 4)),
-                     dim3(256), 0, st, a);
+  hipLaunchKernelGGL((decode_join_kernel<E>), dim3(a.B * a.H), dim3(256), 0, st, a);
   return hipGetLastError();
 }
 

@@ -14,7 +14,7 @@
 //   dQ: 128 queries of one head, looping over key tiles; a query per lane.
 // S and dP are formed twice, 7 products where 5 would do, in exchange for no
 // atomics on dQ.  Tiles without a visible pair are not visited, as in the forward
-// (tile_walk).  An item that would be too long a chain for the size of the launch is
+// (TileWalk).  An item that would be too long a chain for the size of the launch is
 // split into parts (bwd_parts), whose fp32 sums a last launch adds up in order.
 //
 // delta subtracts from dP what O says, so O's rounding would reach every dz of a
@@ -50,22 +50,8 @@ __device__ __forceinline__ void load_own(const TensorArg& t, int b, int h, int r
     x[ks] = valid && 2 * ks + g < dch ? *(const u32x4*)(p + 16 * (2 * ks + g)) : u32x4{0, 0, 0, 0};
 }
 
-// P and the factor of dx that the cap's derivative brings.
-template <typename E, bool CAP, bool BIAS>
-__device__ __forceinline__ float prob(float s, float dist, float slope2, float lse2,
-                                      const ScoreConst& k, float& deriv) {
-  if constexpr (!CAP && !BIAS) {
-    return fast_exp2(__builtin_fmaf(s, k.c, -lse2));
-  } else {
-    float t;
-    const float x = score<E, CAP, BIAS>(s, dist, slope2, k, t);
-    if constexpr (CAP) deriv = __builtin_fmaf(-t, t, 1.f);
-    return fast_exp2(x - lse2);
-  }
-}
-
 // ---------------------------------------------------------------------------
-// delta and lse * log2(e)
+// delta, and lse * log2(e) less the scores' constant
 // ---------------------------------------------------------------------------
 // Eight lanes per row of 16-byte chunks.
 template <typename E>
@@ -99,7 +85,7 @@ __global__ __launch_bounds__(256) void sattn_delta_kernel(SAttnArgs a, uint32_t 
   sum = group_sum<8>(sum);
   if (row < rows && sub == 0) {
     const_cast<float*>(a.delta)[row] = sum;
-    const_cast<float*>(a.lse2)[row] = a.lse[row] * kLog2e;
+    const_cast<float*>(a.lse2)[row] = a.lse[row] * kLog2e - a.sc.b0;
   }
 }
 
@@ -111,7 +97,7 @@ struct Buffers {
   char *A0, *A1, *B0, *B1;
   float *S0, *S1;  // lse2, delta, document ids; for dQ: document ids
   char* own;
-  int* list;       // see tile_walk
+  int* list;       // see TileWalk
 };
 
 template <typename E, int D, bool CAP, bool BIAS>
@@ -161,20 +147,17 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   DocRange own = {0, 0, false};
   if (docs) own = doc_range(docs, k0, kmax - k0 + 1, lane);
   const DocTile* qtiles = a.qtiles + (int64_t)b * ((Sq + 63) / 64);
-  auto look = [&](int t) __attribute__((always_inline)) {
-    const int q0 = t * T, p0 = a.off + q0, p1 = a.off + min(q0 + T, Sq) - 1;
-    bool live = !a.causal || p1 >= k0 || k0 < prefix;
-    bool full = q0 + T <= Sq && (!a.causal || p0 >= kmax || kmax < prefix);
-    bool pad = false;
-    if (docs) {
-      const DocTile w = qtiles[q0 >> 6];
-      live = live && w.lo <= own.hi && w.hi >= own.lo;
-      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
-      pad = w.pad;
-    }
-    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
-  };
   const int nqt = (Sq + T - 1) / T;
+  // first query that sees a key of the workgroup, and the first that sees all of them
+  const int qlive = a.causal && k0 >= prefix ? max(k0 - a.off, 0) : 0;
+  const int qfull = a.causal && kmax >= prefix ? max(kmax - a.off, 0) : 0;
+  auto look = [&](int t) __attribute__((always_inline)) {
+    const DocTile w = qtiles[t * T >> 6];
+    const bool live = (t + 1) * T > qlive && w.lo <= own.hi && w.hi >= own.lo;
+    const bool full = t * T >= qfull && (t + 1) * T <= Sq && w.lo == w.hi && own.lo == own.hi &&
+                      w.lo == own.lo && !w.pad && !own.pad;
+    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
+  };
   Stage<E, D, T> qsrc, gsrc;
   qsrc.init(a.q, b, 0, a.dch, lane, wave);
   gsrc.init(a.dout, b, 0, a.dch, lane, wave);
@@ -205,6 +188,8 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   for (int i = 0; i < L::DB; ++i) dk[i] = dv[i] = f32x16{};
 
   float slope2 = 0.f;
+  // with a causal mask alone no visible key is ahead of its query
+  const bool one_sided = BIAS && a.causal && !a.prefix;
   auto step = [&](int cur, int nxt, int hnext, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
     const char* qt = I ? Q1 : Q0;
@@ -232,20 +217,30 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks)
           dp = Elem<E>::mfma(rd.row(gt, qb, ks), vn[ks], dp);
-        // query of register r: q0 + 32 qb + 8 (r / 4) + 4 g + r % 4
-        const float d0 = (float)(p0 - krow + 32 * qb + 4 * g);
+        // query of register r: q0 + 32 qb + 8 (r / 4) + 4 g + r % 4, d0 + 8 (r / 4) + r % 4
+        // ahead of the lane's key
+        const float d0 = (float)(p0 - krow + 32 * qb + 4 * g), base = -slope2 * d0;
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
           const f32x4 l4 = *(const f32x4*)(st + 32 * qb + 8 * jj + 4 * g);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = 4 * jj + i;
-            float deriv = 1.f;
-            const float p =
-                prob<E, CAP, BIAS>(s[r], d0 + (8 * jj + i), slope2, l4[i], a.sc, deriv);
+            const float y = score_y<E, CAP>(s[r], a.sc);
+            float x;
+            if constexpr (BIAS) {
+              if (one_sided)
+                x = __builtin_fmaf(y, a.sc.f, base - __builtin_fmaf(slope2, 8 * jj + i, l4[i]));
+              else
+                x = __builtin_fmaf(y, a.sc.f, __builtin_fmaf(
+                        -slope2, __builtin_fabsf(d0 + (8 * jj + i)), -l4[i]));
+            } else {
+              x = __builtin_fmaf(y, a.sc.f, -l4[i]);
+            }
+            const float p = fast_exp2(x);
             s[r] = p;
             dp[r] = -(p * dp[r]);
-            if constexpr (CAP) dp[r] *= deriv;
+            if constexpr (CAP) dp[r] *= score_slope<E, CAP>(y);
           }
         }
         if (!full) {
@@ -288,7 +283,18 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   };
   // the group's query heads one after another
   for (int first = 0; first < nqt; first += kListed) {
-    TileWalk walk = tile_walk(buf.list, first, nqt, part, a.parts, hk * a.G, a.G, look);
+    TileWalk walk;
+    if (docs) {
+      walk.list = buf.list;
+      walk.count = tile_list(buf.list, first, nqt, look);
+    } else {
+      walk.list = nullptr;
+      walk.lo = max(first, qlive / T);
+      walk.f0 = (qfull + T - 1) / T;
+      walk.f1 = Sq / T;
+      walk.count = min(nqt, first + kListed) - walk.lo;
+    }
+    walk.begin(part, a.parts, hk * a.G, a.G);
     int cur = walk.entry();
     if (cur >= 0) fetch(cur, walk.head, Q0, G0, S0);
     __syncthreads();
@@ -367,18 +373,13 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + 63) / 64);
   const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + T - 1) / T;
+  const int kfull = a.causal ? min(max(pmin + 1, prefix), Sk) : Sk;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const int k0 = t * T;
-    bool live = !a.causal || k0 <= pmax || k0 < prefix;
-    bool full = k0 + T <= Sk && (!a.causal || k0 + T - 1 <= pmin || k0 + T <= prefix);
-    bool pad = false;
-    if (docs) {
-      const DocTile w = ktiles[k0 >> 6];
-      live = live && w.lo <= own.hi && w.hi >= own.lo;
-      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
-      pad = w.pad;
-    }
-    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
+    const DocTile w = ktiles[t * T >> 6];
+    const bool live = w.lo <= own.hi && w.hi >= own.lo;
+    const bool full = (t + 1) * T <= kfull && w.lo == w.hi && own.lo == own.hi &&
+                      w.lo == own.lo && !w.pad && !own.pad;
+    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
   };
 
   Stage<E, D, T> ksrc, vsrc;
@@ -402,6 +403,7 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   f32x16 acc[L::DB];
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  const bool one_sided = BIAS && a.causal && !a.prefix;
   auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
     const char* kt = I ? K1 : K0;
@@ -423,13 +425,23 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks) dp = Elem<E>::mfma(rd.row(vt, kb, ks), df[ks], dp);
         const float d0 = (float)(qpos - k0 - 32 * kb - 4 * g);
+        const float base = -__builtin_fmaf(slope2, d0, lse2);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          float deriv = 1.f;
-          const float p = prob<E, CAP, BIAS>(s[r], d0 - (8 * (r >> 2) + (r & 3)), slope2, lse2, a.sc,
-                                             deriv);
-          dp[r] *= p;
-          if constexpr (CAP) dp[r] *= deriv;
+          const float y = score_y<E, CAP>(s[r], a.sc);
+          float x;
+          if constexpr (BIAS) {
+            // the key is d0 - n behind its query, n = 8 (r / 4) + r % 4
+            if (one_sided)
+              x = __builtin_fmaf(y, a.sc.f, slope2 * (float)(r & 3)) + (base + slope2 * (8 * (r >> 2)));
+            else
+              x = __builtin_fmaf(y, a.sc.f, __builtin_fmaf(
+                      -slope2, __builtin_fabsf(d0 - (8 * (r >> 2) + (r & 3))), -lse2));
+          } else {
+            x = __builtin_fmaf(y, a.sc.f, -lse2);
+          }
+          dp[r] *= fast_exp2(x);
+          if constexpr (CAP) dp[r] *= score_slope<E, CAP>(y);
         }
         if (!(cur & kFull)) {
           const int rel = klast - k0 - 32 * kb - 4 * g;
@@ -460,7 +472,17 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
     __syncthreads();
   };
   for (int first = 0; first < ntiles; first += kListed) {
-    TileWalk walk = tile_walk(buf.list, first, ntiles, part, a.qparts, 0, 1, look);
+    TileWalk walk;
+    if (docs) {
+      walk.list = buf.list;
+      walk.count = tile_list(buf.list, first, ntiles, look);
+    } else {
+      walk.list = nullptr;
+      walk.lo = walk.f0 = first;
+      walk.f1 = kfull / T;
+      walk.count = min(ntiles - first, kListed);
+    }
+    walk.begin(part, a.qparts, 0, 1);
     int cur = walk.entry();
     if (cur >= 0) fetch(cur, K0, V0, I0);
     __syncthreads();

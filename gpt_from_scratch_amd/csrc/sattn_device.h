@@ -199,50 +199,45 @@ struct Stage {
   }
 };
 
-// Scores.  x is in log2 units (times log2(e)) wherever a cap or a bias makes it;
-// without either the raw product stays and kRaw's factor goes into the exp2.
+// Scores in log2 units: x = f * y + b0 - slope2 * |i - j| of y, the raw product s or
+// what the cap makes of it.
 struct ScoreConst {
-  float c;       // scale * log2(e)
-  float k1;      // 2 * log2(e) * scale / cap
-  float kz;      // scale / cap
-  float capl2;   // cap * log2(e)
+  float f, b0;
+  float k1;  // cap: 2 * log2(e) * scale / cap
+  float kz;  // cap: scale / cap
 };
 
-// tanh(z / cap) of a raw product s.  16-bit inputs: 1 - 2 / (1 + exp(2 y)), which
-// is off by about 1e-7 absolutely, cap * 1e-7 in the score, far below the
-// rounding of P.  fp32: the Taylor series below |y| = 0.4 (7 terms, next one
-// 4e-9), where that formula loses the leading digits.
-template <typename E>
-__device__ __forceinline__ float cap_tanh(float s, const ScoreConst& k) {
-  const float r = __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k.k1));
-  const float t = __builtin_fmaf(-2.f, r, 1.f);
-  if constexpr (Elem<E>::kBytes == 2) {
-    return t;
+// y with a cap: tanh(z) = 1 - 2 / (1 + exp(2 z)).
+//   16-bit inputs: y = -1 / (1 + exp(2 z)), f = 2 cap log2(e), b0 = cap log2(e): one
+//   multiply-add fewer per score.  Off by about 1e-7 absolutely, cap * 1e-7 in the
+//   score, far below the rounding of P.
+//   fp32: y = tanh(z), f = cap log2(e), b0 = 0, by the Taylor series below |z| = 0.4
+//   (7 terms, the next one 4e-9), where the formula loses the leading digits.
+template <typename E, bool CAP>
+__device__ __forceinline__ float score_y(float s, const ScoreConst& k) {
+  if constexpr (!CAP) {
+    return s;
+  } else if constexpr (Elem<E>::kBytes == 2) {
+    return __builtin_amdgcn_rcpf(-1.f - fast_exp2(s * k.k1));
   } else {
-    const float y = s * k.kz, u = y * y;
+    const float t =
+        __builtin_fmaf(-2.f, __builtin_amdgcn_rcpf(1.f + fast_exp2(s * k.k1)), 1.f);
+    const float z = s * k.kz, u = z * z;
     float p = __builtin_fmaf(u, 21844.f / 6081075.f, -1382.f / 155925.f);
     p = __builtin_fmaf(u, p, 62.f / 2835.f);
     p = __builtin_fmaf(u, p, -17.f / 315.f);
     p = __builtin_fmaf(u, p, 2.f / 15.f);
     p = __builtin_fmaf(u, p, -1.f / 3.f);
-    p = __builtin_fmaf(u * p, y, y);
+    p = __builtin_fmaf(u * p, z, z);
     return u < 0.16f ? p : t;
   }
 }
-
-// x of raw product s; dist = |i - j| (as float, any sign), slope2 = slope * log2(e).
-template <typename E, bool CAP, bool BIAS>
-__device__ __forceinline__ float score(float s, float dist, float slope2, const ScoreConst& k,
-                                       float& t) {
-  float x = s;
-  if constexpr (CAP) {
-    t = cap_tanh<E>(s, k);
-    x = k.capl2 * t;
-  } else if constexpr (BIAS) {
-    x = s * k.c;
-  }
-  if constexpr (BIAS) x = __builtin_fmaf(-slope2, __builtin_fabsf(dist), x);
-  return x;
+// d score / d raw product, over scale: 1 - tanh^2.
+template <typename E, bool CAP>
+__device__ __forceinline__ float score_slope(float y) {
+  if constexpr (!CAP) return 1.f;
+  else if constexpr (Elem<E>::kBytes == 2) return -4.f * y * (y + 1.f);
+  else return __builtin_fmaf(-y, y, 1.f);
 }
 
 // What 64 rows' document ids say: range of the ids >= 0 (lo > hi: none), whether
@@ -317,20 +312,24 @@ __device__ __forceinline__ DocRange doc_range(const int* ids, int row0, int n, i
   return r;
 }
 
-// The streamed tiles a workgroup has to visit, in order: a list in LDS, built 64
-// tiles at a time (lane t looks at one tile, a ballot gives the live ones their
-// places), at most kListed tiles of the sequence in one list.  An entry is a tile's
-// index with kFull (every pair visible: no mask) and kPad (rows of negative document
-// id in it).  The walk over it, `heads` times for dK / dV, takes the entries part,
+// The streamed tiles a workgroup has to visit, in order.  Without documents a range;
+// with them a list in LDS, built 64 tiles at a time (lane t looks at one tile, a
+// ballot gives the live ones their places), at most kListed tiles of the sequence in
+// one list.  An entry is a tile's index with kFull (every pair visible: no mask) and
+// kPad (rows of negative document id in it).  The walk over it, `heads` times for dK / dV, takes the entries part,
 // part + parts, ...: equal shares whatever the mask.
 constexpr int kFull = 1 << 30, kPad = 1 << 29, kTileIndex = kPad - 1;
 constexpr int kListed = 512;
 
 struct TileWalk {
-  const int* list;
+  const int* list;                 // null: tiles [lo, lo + count), full in [f0, f1)
+  int lo, f0, f1;
   int count, at, parts, head, hend;
   __device__ __forceinline__ int entry() const {  // -1 behind the last
-    return head < hend ? __builtin_amdgcn_readfirstlane(list[at]) : -1;
+    if (head >= hend) return -1;
+    if (list) return __builtin_amdgcn_readfirstlane(list[at]);
+    const int t = lo + at;
+    return t >= f0 && t < f1 ? t | kFull : t;
   }
   __device__ __forceinline__ void step(int n) {
     at += n;
@@ -339,13 +338,19 @@ struct TileWalk {
       ++head;
     }
   }
+  __device__ __forceinline__ void begin(int part, int parts_, int head_, int heads) {
+    at = 0;
+    parts = parts_;
+    hend = head_ + heads;
+    head = count > 0 ? head_ : hend;
+    step(part);
+  }
 };
 
 // Tiles [first, first + kListed) of n; `look` says of one: bit 0 live, kFull, kPad.
 // Ends with a barrier.
 template <typename F>
-__device__ __forceinline__ TileWalk tile_walk(int* list, int first, int n, int part, int parts,
-                                              int head, int heads, F look) {
+__device__ __forceinline__ int tile_list(int* list, int first, int n, F look) {
   const int lane = threadIdx.x & 63, end = min(n, first + kListed);
   int count = 0;
   for (int t0 = first; t0 < end; t0 += 64) {
@@ -356,9 +361,7 @@ __device__ __forceinline__ TileWalk tile_walk(int* list, int first, int n, int p
     count += __popcll(live);
   }
   __syncthreads();
-  TileWalk w = {list, count, 0, parts, count ? head : head + heads, head + heads};
-  if (count) w.step(part);
-  return w;
+  return count;
 }
 
 // A part's accumulators (32 rows of a wave, DB column blocks) in the workspace, as

@@ -11,7 +11,7 @@
 // feeds the second product from the accumulators; 64-key tiles of K and V come
 // in by direct global -> LDS loads, double buffered, one barrier per tile.
 //   * Which key tiles a workgroup visits is listed beforehand
-//     (tile_walk) from positions, the prefix and the 64-key ranges of document
+//     (TileWalk) from positions, the prefix and the 64-key ranges of document
 //     ids: tiles without a visible pair cost nothing, tiles where every pair is
 //     visible run without mask code.
 //   * Query heads that share a key head go to the same XCD (workgroups are dealt
@@ -61,8 +61,12 @@ __device__ __forceinline__ void finish_rows(const SAttnArgs& a, int b, int h, in
 
 constexpr float kSlack = 8.f;  // log2 units a score may exceed the running reference by
 
+// Waves per SIMD the register budget is held to.
+template <typename E, int D, bool BIAS>
+constexpr int kFwdWaves = Lay<E, D>::RB > 256 ? 1 : Lay<E, D>::RB > 128 ? 2 : BIAS ? 3 : 4;
+
 template <typename E, int D, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_kernel(SAttnArgs a) {
+__global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel(SAttnArgs a) {
   using L = Lay<E, D>;
   constexpr int BQ = 128, BK = 64;
   __shared__ __attribute__((aligned(16))) char K0[BK * L::RB];
@@ -111,18 +115,14 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
   if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + BK - 1) / BK);
   const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + BK - 1) / BK;
+  // full: all keys before every query of the workgroup, or in the prefix
+  const int kfull = a.causal ? min(max(pmin + 1, prefix), Sk) : Sk;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const int k0 = t * BK;
-    bool live = !a.causal || k0 <= pmax || k0 < prefix;
-    bool full = k0 + BK <= Sk && (!a.causal || k0 + BK - 1 <= pmin || k0 + BK <= prefix);
-    bool pad = false;
-    if (docs) {
-      const DocTile w = ktiles[t];
-      live = live && w.lo <= own.hi && w.hi >= own.lo;
-      full = full && w.lo == w.hi && own.lo == own.hi && w.lo == own.lo && !w.pad && !own.pad;
-      pad = w.pad;
-    }
-    return (live ? 1 : 0) | (full ? kFull : 0) | (pad ? kPad : 0);
+    const DocTile w = ktiles[t];
+    const bool live = w.lo <= own.hi && w.hi >= own.lo;
+    const bool full = (t + 1) * BK <= kfull && w.lo == w.hi && own.lo == own.hi &&
+                      w.lo == own.lo && !w.pad && !own.pad;
+    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
   };
 
   Stage<E, D, BK> ksrc, vsrc;
@@ -148,8 +148,10 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
   float m_run = -INFINITY, l_run = 0.f;
-  // factor that takes a score to log2 units
-  const float c = CAP || BIAS ? 1.f : a.sc.c;
+  const float c = BIAS ? 1.f : a.sc.f;  // factor of y below
+  // with a causal mask alone no visible key is ahead of its query
+  const bool one_sided = BIAS && a.causal && !a.prefix;
+  const float gstep = one_sided ? slope2 : 0.f;
 
   auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
@@ -166,16 +168,34 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
           s[kb] = Elem<E>::mfma(rd.row(kt, kb, ks), qf[ks], ks == 0 ? f32x16{} : s[kb]);
+      // y: scores as f * y + base (+ the group's step, below) in log2 units
+      float base = a.sc.b0;
       if constexpr (CAP || BIAS) {
-        const float d0 = (float)(qpos - k0 - 4 * g);
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            float t;
-            s[kb][r] = score<E, CAP, BIAS>(s[kb][r], d0 - (32 * kb + 8 * (r >> 2) + (r & 3)), slope2,
-                                           a.sc, t);
-          }
+          for (int r = 0; r < 16; ++r) s[kb][r] = score_y<E, CAP>(s[kb][r], a.sc);
+      }
+      if constexpr (BIAS) {
+        const float d0 = (float)(qpos - k0 - 4 * g);
+        if (one_sided) {
+          // key k0 + 4 g + n (n = 8 m + i) is d0 - n behind: -slope2 d0 goes into the
+          // base, slope2 i into y, slope2 8 m into the group of four registers
+          base -= slope2 * d0;
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[kb][r] = __builtin_fmaf(s[kb][r], a.sc.f, slope2 * (float)(r & 3));
+        } else {
+#pragma unroll
+          for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+              s[kb][r] = __builtin_fmaf(
+                  -slope2, __builtin_fabsf(d0 - (32 * kb + 8 * (r >> 2) + (r & 3))),
+                  s[kb][r] * a.sc.f);
+        }
       }
       if (!(cur & kFull)) {
         const int rel = klast - k0 - 4 * g;
@@ -196,10 +216,22 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
             }
         }
       }
-      float mx = vmax(s[0][0], s[0][1]);
+      float mx;
+      if constexpr (BIAS) {
+        mx = -INFINITY;
 #pragma unroll
-      for (int i = 2; i < 32; i += 2) mx = vmax(vmax(mx, s[i >> 4][i & 15]), s[i >> 4][(i & 15) + 1]);
-      mx = max_halves(mx) * c;
+        for (int m = 0; m < 8; ++m) {
+          const f32x16& x = s[m >> 2];
+          const int r = 4 * (m & 3);
+          mx = vmax(mx, vmax(vmax(x[r], x[r + 1]), vmax(x[r + 2], x[r + 3])) + gstep * (8 * m));
+        }
+      } else {
+        mx = vmax(s[0][0], s[0][1]);
+#pragma unroll
+        for (int i = 2; i < 32; i += 2)
+          mx = vmax(vmax(mx, s[i >> 4][i & 15]), s[i >> 4][(i & 15) + 1]);
+      }
+      mx = max_halves(__builtin_fmaf(mx, c, base));  // (base is the half's own)
       // The reference moves only when a score passes it by more than kSlack:
       // P stays below 2^8, and O and l share the reference whatever it is.
       if (__any(mx > m_run + kSlack)) {
@@ -210,14 +242,18 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
         for (int db = 0; db < L::DB; ++db) acc[db] *= alpha;
         m_run = m_new;
       }
-      const float ref = m_run == -INFINITY ? 0.f : m_run;  // a row that has seen no key yet
+      // (0 for a row that has seen no key yet)
+      const float ref = (m_run == -INFINITY ? 0.f : m_run) - base;
       u32x4 p[2][L::NG];
       float ps[2] = {0.f, 0.f};
 #pragma unroll
       for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-          s[kb][r] = fast_exp2(__builtin_fmaf(s[kb][r], c, -ref));
+          if constexpr (BIAS)
+            s[kb][r] = fast_exp2(s[kb][r] - (ref - gstep * (32 * kb + 8 * (r >> 2))));
+          else
+            s[kb][r] = fast_exp2(__builtin_fmaf(s[kb][r], c, -ref));
           // the sum before P is rounded for the product: lse is an fp32 result
           ps[r & 1] += s[kb][r];
         }
@@ -236,7 +272,17 @@ __global__ __launch_bounds__(256, (Lay<E, D>::RB > 256 ? 1 : 2)) void sattn_fwd_
     __syncthreads();
   };
   for (int first = 0; first < ntiles; first += kListed) {
-    TileWalk walk = tile_walk(list, first, ntiles, part, a.parts, 0, 1, look);
+    TileWalk walk;
+    if (docs) {
+      walk.list = list;
+      walk.count = tile_list(list, first, ntiles, look);
+    } else {
+      walk.list = nullptr;
+      walk.lo = walk.f0 = first;
+      walk.f1 = kfull / BK;
+      walk.count = min(ntiles - first, kListed);
+    }
+    walk.begin(part, a.parts, 0, 1);
     int cur = walk.entry();
     if (cur >= 0) fetch(cur, K0, V0, I0);
     __syncthreads();
