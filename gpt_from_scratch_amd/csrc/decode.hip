@@ -21,8 +21,12 @@ namespace mi {
 
 namespace {
 
+// Waves per workgroup: two, so that two workgroups share a CU (64 KB of tiles each at
+// D = 128; one for fp32) and one streams while the other starts or merges.  Four
+// (one workgroup per CU): 71 against 65 us at B32 H32/8 S <= 4096, lengths of 1/8 to 1.
 template <typename E, int D>
-constexpr int kWaves = Lay<E, D>::RB > 256 ? 2 : 4;  // two tiles of K and V in 160 KB
+constexpr int kWaves = 2;
+constexpr int kMaxParts = 64;  // B1 H16/4 S65536: 33 us; 128 the same, 256 43
 
 template <typename E>
 __device__ __forceinline__ void put(void* p, int64_t i, float x) {
@@ -61,7 +65,8 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
                                              : u32x4{0, 0, 0, 0};
   const float slope2 = BIAS && l32 < nh ? a.slopes[h0 + l32] * kLog2e : 0.f;
 
-  Stage<E, D, TK, NW> ksrc, vsrc;
+  // read once: non-temporal (72 against 77 us at the size above)
+  Stage<E, D, TK, NW, kOnce> ksrc, vsrc;
   ksrc.init(a.k, b, hk, a.dch, lane, wave);
   vsrc.init(a.v, b, hk, a.dch, lane, wave);
   Reads<E, D> rd;
@@ -138,7 +143,8 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
   if (t < t1) step(t, std::integral_constant<int, 0>{});
 
   // Merge the waves: each takes its sums to the common maximum and leaves its
-  // O^T, as [head][D + 1] floats, in a tile buffer (idle, and large enough).
+  // O^T, as [head][D] floats, in a tile buffer (idle, and large enough); element d of
+  // head h sits at d ^ h, so that neither side meets in a bank.
   const float l = sum_halves(l_run);
   if (g == 0) {
     ML[0][wave][l32] = m_run;
@@ -154,20 +160,19 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
   const float f = fast_exp2(m_run - ref);
   // one part: normalised here
   const float fo = a.splits == 1 ? (lt == 0.f ? 0.f : f / lt) : f;
-  float* const mine = (float*)(wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1);
-  static_assert(TK * L::RB >= 32 * (D + 1) * 4, "merge buffers");
+  float* const mine = (float*)(wave == 0 ? K0 : K1);
+  static_assert(NW == 2 && TK * L::RB >= 32 * D * 4, "merge buffers");
 #pragma unroll
   for (int db = 0; db < L::DB; ++db)
 #pragma unroll
     for (int r = 0; r < 16; ++r)
-      mine[l32 * (D + 1) + 32 * db + 8 * (r >> 2) + 4 * g + (r & 3)] = acc[db][r] * fo;
+      mine[l32 * D + ((32 * db + 8 * (r >> 2) + 4 * g + (r & 3)) ^ l32)] = acc[db][r] * fo;
   __syncthreads();
   const int64_t row0 = (int64_t)b * a.H + h0;
   for (int i = tid; i < nh * D; i += 64 * NW) {
-    const int hh = i / D, d = i % D, at = hh * (D + 1) + d;
+    const int hh = i / D, d = i % D, at = hh * D + (d ^ hh);
     if (d >= a.D) continue;
-    float x = ((float*)K0)[at] + ((float*)K1)[at];
-    if constexpr (NW == 4) x += ((float*)V0)[at] + ((float*)V1)[at];
+    const float x = ((float*)K0)[at] + ((float*)K1)[at];
     if (a.splits == 1)
       put<E>(a.o, b * a.o_sb + (h0 + hh) * a.o_sh + d, x);
     else
@@ -180,32 +185,35 @@ __global__ __launch_bounds__((64 * kWaves<E, D>), 1) void decode_kernel(DecodeAr
   }
 }
 
-// O of one row from its parts: a workgroup per row, its waves a quarter of the parts
-// each, lane d, d + 64 (one wave over 64 parts, a chain of 64 loads, took 35 us).
-template <typename E>
-__global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
-  __shared__ float sum[4][128], weight[64];
+// O of one row from its parts: a workgroup of JW waves per row, lane d, d + 64.  The
+// time is each wave's chain of loads (one wave over 64 parts took 35 us), kept to four
+// parts, all in flight: 16 waves, or 4 for up to 16 parts, where many rows would only
+// start waves (B32 H32: 68 against 65 us).
+template <typename E, int JW>
+__global__ __launch_bounds__(64 * JW) void decode_join_kernel(DecodeArgs a) {
+  __shared__ float sum[JW][128], weight[kMaxParts];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t row = blockIdx.x;
-  // splits <= 64: a part per lane
-  float m = -INFINITY, l = 0.f;
-  if (lane < a.splits) {
-    m = a.ml[2 * (row * a.splits + lane)];
-    l = a.ml[2 * (row * a.splits + lane) + 1];
-  }
-  float mt = m;
+  const float* ml = a.ml + 2 * row * a.splits;
+  float mt = -INFINITY;
+  for (int i = lane; i < a.splits; i += 64) mt = fmaxf(mt, ml[2 * i]);
 #pragma unroll
   for (int x = 32; x; x >>= 1) mt = fmaxf(mt, __shfl_xor(mt, x, 64));
-  const float f = fast_exp2(m - (mt == -INFINITY ? 0.f : mt));
-  float lt = l * f;
+  float lt = 0.f;
+  for (int i = lane; i < a.splits; i += 64) {
+    const float f = fast_exp2(ml[2 * i] - (mt == -INFINITY ? 0.f : mt));
+    lt = __builtin_fmaf(ml[2 * i + 1], f, lt);
+    if (wave == 0) weight[i] = f;
+  }
 #pragma unroll
   for (int x = 32; x; x >>= 1) lt += __shfl_xor(lt, x, 64);
-  if (wave == 0) weight[lane] = f;
   __syncthreads();
   const float* part = a.part + row * a.splits * a.D;
   float o0 = 0.f, o1 = 0.f;
-#pragma unroll 8
-  for (int s = wave; s < a.splits; s += 4) {
+#pragma unroll
+  for (int n = 0; n < 4; ++n) {
+    const int s = wave + JW * n;
+    if (s >= a.splits) break;
     const float w = weight[s];
     if (lane < a.D) o0 = __builtin_fmaf(part[s * a.D + lane], w, o0);
     if (lane + 64 < a.D) o1 = __builtin_fmaf(part[s * a.D + lane + 64], w, o1);
@@ -215,7 +223,9 @@ __global__ __launch_bounds__(256) void decode_join_kernel(DecodeArgs a) {
   __syncthreads();
   const int d = threadIdx.x;
   if (d >= a.D) return;
-  const float o = (sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d]);
+  float o = 0.f;
+#pragma unroll
+  for (int w = 0; w < JW; ++w) o += sum[w][d];
   put<E>(a.o, row / a.H * a.o_sb + row % a.H * a.o_sh + d, lt == 0.f ? 0.f : o / lt);
 }
 
@@ -232,7 +242,11 @@ hipError_t launch_d(const DecodeArgs& a, bool cap, hipStream_t st) {
     hipLaunchKernelGGL((decode_kernel<E, D, false, false>), grid, block, 0, st, a);
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.splits == 1) return e;
-  hipLaunchKernelGGL((decode_join_kernel<E>), dim3(a.B * a.H), dim3(256), 0, st, a);
+  static_assert(kMaxParts == 64, "four parts to a wave");
+  if (a.splits <= 16)
+    hipLaunchKernelGGL((decode_join_kernel<E, 4>), dim3(a.B * a.H), dim3(256), 0, st, a);
+  else
+    hipLaunchKernelGGL((decode_join_kernel<E, 16>), dim3(a.B * a.H), dim3(1024), 0, st, a);
   return hipGetLastError();
 }
 
@@ -243,14 +257,13 @@ hipError_t launch_e(const DecodeArgs& a, bool cap, hipStream_t st) {
 
 }  // namespace
 
-// Parts the keys are split into: enough workgroups for two per CU, at least two
-// tiles (of 128 keys, 64 for fp32 rows past 256 bytes) to a part.
+// Parts the keys are split into: four workgroups per CU, so that sequences of
+// different lengths even out, at least four tiles of 64 keys to a part.
 int decode_splits(int dtype, int B, int H, int Hk, int S, int D) {
-  const int tile = dtype == 0 && D > 64 ? 64 : 128;
   const int64_t wgs = (int64_t)B * Hk * ((H / Hk + 31) / 32);
-  const int64_t want = (512 + wgs - 1) / wgs, most = (S + 2 * tile - 1) / (2 * tile);
+  const int64_t want = (1024 + wgs - 1) / wgs, most = ((int64_t)S + 255) / 256;
   const int64_t n = want < most ? want : most;
-  return n < 1 ? 1 : n > 64 ? 64 : (int)n;
+  return n > kMaxParts ? kMaxParts : (int)n;
 }
 
 hipError_t launch_decode(int dtype, const DecodeArgs& a, bool cap, hipStream_t st) {

@@ -149,7 +149,14 @@ struct Reads {
 // Fills ROWS-row tiles from a [rows, D] tensor with direct global -> LDS loads:
 // wave w fills slices w, w + NW, ...  Chunks at or past the tensor's head dim
 // and rows at or past `rows` arrive as zeros.
-template <typename E, int D, int ROWS, int NW = 4>
+// AUX: cache policy of the loads (0, or kOnce for what nothing reads again).
+constexpr int kOnce = 2;  // non-temporal
+template <int AUX>
+__device__ __forceinline__ void load_lds16(__amdgpu_buffer_rsrc_t rs, uint32_t off, char* lds) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (__attribute__((address_space(3))) void*)lds, 16,
+                                           off, 0, 0, AUX);
+}
+template <typename E, int D, int ROWS, int NW = 4, int AUX = 0>
 struct Stage {
   using L = Lay<E, D>;
   static constexpr int SPW = ROWS * L::RB / 1024 / NW;
@@ -179,7 +186,7 @@ struct Stage {
     const auto rs = tile_rsrc(base + row0 * sb, (uint32_t)((rows - 1) * (int)sb) + tail);
 #pragma unroll
     for (int m = 0; m < SPW; ++m)
-      buffer_load_lds16(rs, off[m], (uint16_t*)(tile + (wave + NW * m) * 1024));
+      load_lds16<AUX>(rs, off[m], tile + (wave + NW * m) * 1024);
   }
   // The same with rows of negative document id as zeros too (their contents may
   // be anything, and 0 * NaN is not 0).  ids: of row row0 and on.
@@ -195,7 +202,7 @@ struct Stage {
     }
 #pragma unroll
     for (int m = 0; m < SPW; ++m)
-      buffer_load_lds16(rs, o[m], (uint16_t*)(tile + (wave + NW * m) * 1024));
+      load_lds16<AUX>(rs, o[m], tile + (wave + NW * m) * 1024);
   }
 };
 
