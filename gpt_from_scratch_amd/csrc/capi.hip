@@ -1431,9 +1431,9 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
   a.olo = o_lo;
   a.lse = lse;
   if (((uintptr_t)o_lo) % 16) return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-byte aligned rows wanted");
-  if ((st = check_workspace(workspace, workspace_elems, mi::sattn_fwd_workspace(a))) != MI_OK)
-    return st;
-  mi::sattn_fwd_split(a, workspace);
+  int64_t want = 0;
+  mi::sattn_fwd_split(dtype, a, workspace, &want);
+  if ((st = check_workspace(workspace, workspace_elems, want)) != MI_OK) return st;
   if (a.docs) {
     st = launched(mi::launch_doc_tiles(a.docs, tiles, B, Sq, Sk, (hipStream_t)stream), "doc_tiles");
     if (st != MI_OK) return st;
@@ -1444,7 +1444,16 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
 
 int64_t mi_sattn_fwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
   if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
-  return mi::sattn_fwd_workspace(sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr));
+  int64_t most = 0;
+  for (int causal = 0; causal < 2; ++causal) {  // the split depends on it
+    mi_score_mods mods = {};
+    mods.causal = causal;
+    mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, mods, nullptr);
+    int64_t n = 0;
+    mi::sattn_fwd_split(dtype, a, nullptr, &n);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {

@@ -198,10 +198,8 @@ struct SAttnArgs;
 struct DecodeArgs;
 hipError_t launch_doc_tiles(const int* docs, void* tiles, int B, int Sq, int Sk, hipStream_t st);
 hipError_t launch_sattn_fwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st);
-// Floats of workspace of the forward, and how the call uses them.
-int64_t sattn_fwd_workspace(const SAttnArgs& a);
-void sattn_fwd_split(SAttnArgs& a, float* ws);
-// The same for the backward (elems may be null).
+// Floats of workspace (elems may be null) and how a call uses them.
+void sattn_fwd_split(int dtype, SAttnArgs& a, float* ws, int64_t* elems);
 void sattn_bwd_split(SAttnArgs& a, float* ws, int64_t* elems);
 hipError_t launch_sattn_bwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st);
 int decode_splits(int dtype, int B, int H, int Hk, int S, int D);

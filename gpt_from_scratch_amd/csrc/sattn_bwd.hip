@@ -201,9 +201,10 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
     if (wave_valid && p0 + T - 1 >= wfirst) {
       const bool full = cur & kFull;
       u32x4 pb[TB][L::NG], sb[TB][L::NG];
+      f32x16 ss[TB], dps[TB];
 #pragma unroll
       for (int qb = 0; qb < TB; ++qb) {
-        f32x16 s, dp;
+        f32x16 &s = ss[qb], &dp = dps[qb];
 #pragma unroll
         for (int jj = 0; jj < 4; ++jj) {
           const f32x4 d4 = *(const f32x4*)(st + T + 32 * qb + 8 * jj + 4 * g);
@@ -217,6 +218,10 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks)
           dp = Elem<E>::mfma(rd.row(gt, qb, ks), vn[ks], dp);
+      }
+#pragma unroll
+      for (int qb = 0; qb < TB; ++qb) {
+        f32x16 &s = ss[qb], &dp = dps[qb];
         // query of register r: q0 + 32 qb + 8 (r / 4) + 4 g + r % 4, d0 + 8 (r / 4) + r % 4
         // ahead of the lane's key
         const float d0 = (float)(p0 - krow + 32 * qb + 4 * g), base = -slope2 * d0;
@@ -314,9 +319,9 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
 
   if (!wave_valid) return;
   if (a.parts > 1) {
-    const int64_t at = 2 * (((int64_t)kt * BHk + bk) * a.parts + part);
-    part_store<L::DB>(dv, part_at<L::DB>(a.part, at, wave), lane);
-    part_store<L::DB>(dk, part_at<L::DB>(a.part, at + 1, wave), lane);
+    const int64_t at = 2 * (((int64_t)(kw / 32) * BHk + bk) * a.parts + part);
+    part_store<L::DB>(dv, part_at<L::DB>(a.part, at), lane);
+    part_store<L::DB>(dk, part_at<L::DB>(a.part, at + 1), lane);
     return;
   }
   // idle now: the wave's K rows, or one of the tile buffers
@@ -414,9 +419,10 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
     const int k0 = (cur & kTileIndex) * T;
     if (wave_valid && k0 <= wlast) {
       u32x4 sb[TB][L::NG];
+      f32x16 ss[TB], dps[TB];
 #pragma unroll
       for (int kb = 0; kb < TB; ++kb) {
-        f32x16 s, dp;
+        f32x16 &s = ss[kb], &dp = dps[kb];
 #pragma unroll
         for (int r = 0; r < 16; ++r) dp[r] = ndelta;
 #pragma unroll
@@ -424,6 +430,10 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
           s = Elem<E>::mfma(rd.row(kt, kb, ks), qf[ks], ks == 0 ? f32x16{} : s);
 #pragma unroll
         for (int ks = 0; ks < L::KS; ++ks) dp = Elem<E>::mfma(rd.row(vt, kb, ks), df[ks], dp);
+      }
+#pragma unroll
+      for (int kb = 0; kb < TB; ++kb) {
+        f32x16 &s = ss[kb], &dp = dps[kb];
         const float d0 = (float)(qpos - k0 - 32 * kb - 4 * g);
         const float base = -__builtin_fmaf(slope2, d0, lse2);
 #pragma unroll
@@ -500,8 +510,8 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
 
   if (!wave_valid) return;
   if (a.qparts > 1) {
-    const int64_t at = ((int64_t)qt * BH + b * a.H + h) * a.qparts + part;
-    part_store<L::DB>(acc, part_at<L::DB>(a.qpart, at, wave), lane);
+    const int64_t at = ((int64_t)(qw / 32) * BH + b * a.H + h) * a.qparts + part;
+    part_store<L::DB>(acc, part_at<L::DB>(a.qpart, at), lane);
     return;
   }
   char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
@@ -554,13 +564,13 @@ __global__ __launch_bounds__(256) void sattn_sum_kernel(SAttnArgs a, int n0) {
   f32x16 acc[L::DB];
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
+  const int64_t at = (int64_t)(row / 32) * n + bh;
   if (query) {
     for (int i = 0; i < a.qparts; ++i)
-      part_add<L::DB>(acc, part_at<L::DB>(a.qpart, (int64_t)which * a.qparts + i, wave), lane, 1.f);
+      part_add<L::DB>(acc, part_at<L::DB>(a.qpart, at * a.qparts + i), lane, 1.f);
   } else {
     for (int i = 0; i < a.parts; ++i)
-      part_add<L::DB>(acc, part_at<L::DB>(a.part, 2 * ((int64_t)which * a.parts + i) + second, wave),
-                      lane, 1.f);
+      part_add<L::DB>(acc, part_at<L::DB>(a.part, 2 * (at * a.parts + i) + second), lane, 1.f);
   }
   const TensorArg& t = query ? a.dq : second ? a.dk : a.dv;
   store_rows<E, D>(acc, query || second ? a.scale : 1.f, stage[wave],
@@ -606,7 +616,7 @@ hipError_t launch_e(const SAttnArgs& a, bool cap, hipStream_t st) {
 // Parts of items of `steps` streamed tiles each, when there are n of them: a chain as
 // long as the launch has room for, at least four tiles to a part.
 int parts_of(int64_t n, int64_t steps) {
-  const int64_t most = (steps + 3) / 4, want = 1024 / n;
+  const int64_t most = (steps + 3) / 4, want = 512 / n;
   return (int)(want < 2 ? 1 : want < most ? want : most);
 }
 

@@ -100,7 +100,8 @@ struct Reads {
   static constexpr int NR = L::KS < 8 ? L::KS : 8;          // beyond: + 256 bytes
   static constexpr int NT = L::ESZ == 4 ? 4 : 2 * L::DB;
   int r[NR], t[NT];
-  __device__ __forceinline__ void init(int lane) {
+  // `block`: the 32-row block that block 0 below stands for.
+  __device__ __forceinline__ void init(int lane, int block = 0) {
     const int l32 = lane & 31, g = lane >> 5;
 #pragma unroll
     for (int ks = 0; ks < NR; ++ks) r[ks] = l32 * L::RB + (((2 * ks + g) ^ L::swz(l32)) << 4);
@@ -118,6 +119,10 @@ struct Reads {
           t[2 * db + h] = (row + 8 * h) * L::RB + (((4 * db + ch) ^ L::swz(row + 8 * h)) << 4) +
                           8 * (lane & 1);
     }
+#pragma unroll
+    for (int i = 0; i < NR; ++i) r[i] += 32 * block * L::RB;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) t[i] += 32 * block * L::RB;
   }
   __device__ __forceinline__ void refresh() {
 #pragma unroll
@@ -371,12 +376,11 @@ __device__ __forceinline__ int tile_list(int* list, int first, int n, F look) {
   return count;
 }
 
-// A part's accumulators (32 rows of a wave, DB column blocks) in the workspace, as
-// they lie in the registers: whole 1 KB stores and loads.  `index`: which tile,
-// tensor and part.
+// A part's accumulators (32 rows, DB column blocks) in the workspace, as they lie in
+// the registers: whole 1 KB stores and loads.  `index`: which rows, tensor and part.
 template <int DB>
-__device__ __forceinline__ f32x4* part_at(float* part, int64_t index, int wave) {
-  return (f32x4*)(part + (index * 4 + wave) * (DB * 1024));
+__device__ __forceinline__ f32x4* part_at(float* part, int64_t index) {
+  return (f32x4*)(part + index * (DB * 1024));
 }
 template <int DB>
 __device__ __forceinline__ void part_store(const f32x16 (&acc)[DB], f32x4* p, int lane) {

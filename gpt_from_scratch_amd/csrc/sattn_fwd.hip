@@ -65,10 +65,12 @@ constexpr float kSlack = 8.f;  // log2 units a score may exceed the running refe
 template <typename E, int D, bool BIAS>
 constexpr int kFwdWaves = Lay<E, D>::RB > 256 ? 1 : Lay<E, D>::RB > 128 ? 2 : BIAS ? 3 : 4;
 
-template <typename E, int D, bool CAP, bool BIAS>
+// KS = 2: a wave takes one 32-key block of each tile instead of both, two waves share
+// 32 query rows and merge at the end, and a workgroup owns 64 rows (see key_split).
+template <typename E, int D, bool CAP, bool BIAS, int KS>
 __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel(SAttnArgs a) {
   using L = Lay<E, D>;
-  constexpr int BQ = 128, BK = 64;
+  constexpr int BQ = 128 / KS, BK = 64, NB = 2 / KS;
   __shared__ __attribute__((aligned(16))) char K0[BK * L::RB];
   __shared__ __attribute__((aligned(16))) char K1[BK * L::RB];
   __shared__ __attribute__((aligned(16))) char V0[BK * L::RB];
@@ -89,7 +91,8 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   const int n = blockIdx.x % BH, bk = n % BHk, b = bk / a.Hk, hk = bk % a.Hk;
   const int h = hk * a.G + n / BHk;
 
-  const int q0 = qt * BQ, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
+  const int q0 = qt * BQ, qw = q0 + 32 * (wave / KS), qrow = qw + l32, qpos = a.off + qrow;
+  const int slice = KS == 1 ? 0 : wave & 1;
   const bool wave_valid = qw < Sq;
   const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
   const int prefix = a.prefix ? a.prefix[b] : 0;
@@ -129,7 +132,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   ksrc.init(a.k, b, hk, a.dch, lane, wave);
   vsrc.init(a.v, b, hk, a.dch, lane, wave);
   Reads<E, D> rd;
-  rd.init(lane);
+  rd.init(lane, slice);
 
   auto fetch = [&](int t, char* kb, char* vb, int* ib) __attribute__((always_inline)) {
     const int k0 = (t & kTileIndex) * BK;
@@ -160,19 +163,19 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
     const int* it = I ? I1 : I0;
     if (nxt >= 0) fetch(nxt, I ? K0 : K1, I ? V0 : V1, I ? I0 : I1);
     rd.refresh();
-    const int k0 = (cur & kTileIndex) * BK;
+    const int k0 = (cur & kTileIndex) * BK + 32 * slice;  // the wave's first key
     if (wave_valid && k0 <= wlast) {
-      f32x16 s[2];
+      f32x16 s[NB];
 #pragma unroll
       for (int ks = 0; ks < L::KS; ++ks)
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
           s[kb] = Elem<E>::mfma(rd.row(kt, kb, ks), qf[ks], ks == 0 ? f32x16{} : s[kb]);
       // y: scores as f * y + base (+ the group's step, below) in log2 units
       float base = a.sc.b0;
       if constexpr (CAP || BIAS) {
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) s[kb][r] = score_y<E, CAP>(s[kb][r], a.sc);
       }
@@ -183,13 +186,13 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
           // base, slope2 i into y, slope2 8 m into the group of four registers
           base -= slope2 * d0;
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               s[kb][r] = __builtin_fmaf(s[kb][r], a.sc.f, slope2 * (float)(r & 3));
         } else {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int r = 0; r < 16; ++r)
               s[kb][r] = __builtin_fmaf(
@@ -200,16 +203,16 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
       if (!(cur & kFull)) {
         const int rel = klast - k0 - 4 * g;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (32 * kb + 8 * (r >> 2) + (r & 3) > rel) s[kb][r] = -INFINITY;
         if (docs) {
 #pragma unroll
-          for (int kb = 0; kb < 2; ++kb)
+          for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
-              const i32x4 d4 = *(const i32x4*)(it + 32 * kb + 8 * jj + 4 * g);
+              const i32x4 d4 = *(const i32x4*)(it + 32 * (slice + kb) + 8 * jj + 4 * g);
 #pragma unroll
               for (int i = 0; i < 4; ++i)
                 if (d4[i] != qdoc) s[kb][4 * jj + i] = -INFINITY;
@@ -220,7 +223,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
       if constexpr (BIAS) {
         mx = -INFINITY;
 #pragma unroll
-        for (int m = 0; m < 8; ++m) {
+        for (int m = 0; m < 4 * NB; ++m) {
           const f32x16& x = s[m >> 2];
           const int r = 4 * (m & 3);
           mx = vmax(mx, vmax(vmax(x[r], x[r + 1]), vmax(x[r + 2], x[r + 3])) + gstep * (8 * m));
@@ -228,7 +231,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
       } else {
         mx = vmax(s[0][0], s[0][1]);
 #pragma unroll
-        for (int i = 2; i < 32; i += 2)
+        for (int i = 2; i < 16 * NB; i += 2)
           mx = vmax(vmax(mx, s[i >> 4][i & 15]), s[i >> 4][(i & 15) + 1]);
       }
       mx = max_halves(__builtin_fmaf(mx, c, base));  // (base is the half's own)
@@ -244,10 +247,10 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
       }
       // (0 for a row that has seen no key yet)
       const float ref = (m_run == -INFINITY ? 0.f : m_run) - base;
-      u32x4 p[2][L::NG];
+      u32x4 p[NB][L::NG];
       float ps[2] = {0.f, 0.f};
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
+      for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           if constexpr (BIAS)
@@ -262,7 +265,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
       }
       l_run += ps[0] + ps[1];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
         for (int ng = 0; ng < L::NG; ++ng)
 #pragma unroll
@@ -298,13 +301,34 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
     }
   }
 
-  if (!wave_valid) return;
-  const float l = sum_halves(l_run);
+  float l = sum_halves(l_run);
   char* stage = wave == 0 ? K0 : wave == 1 ? K1 : wave == 2 ? V0 : V1;
+  if constexpr (KS > 1) {
+    // the second wave of a pair hands over, the first takes both to the common reference
+    __shared__ float ml[2][2][64];
+    float* const other = (float*)(wave < 2 ? K0 : K1);
+    float(&pml)[2][64] = ml[wave >> 1];
+    if (slice) {
+      part_store<L::DB>(acc, (f32x4*)other, lane);
+      pml[0][lane] = m_run;
+      pml[1][lane] = l;
+    }
+    __syncthreads();
+    if (slice) return;
+    const float m1 = pml[0][lane], m = fmaxf(m_run, m1), ref = m == -INFINITY ? 0.f : m;
+    const float f0 = fast_exp2(m_run - ref), f1 = fast_exp2(m1 - ref);
+#pragma unroll
+    for (int db = 0; db < L::DB; ++db) acc[db] *= f0;
+    part_add<L::DB>(acc, (const f32x4*)other, lane, f1);
+    l = __builtin_fmaf(l, f0, pml[1][lane] * f1);
+    m_run = m;
+    stage = wave == 0 ? V0 : V1;
+  }
+  if (!wave_valid) return;
   if (a.parts > 1) {
-    const int64_t at = ((int64_t)qt * BH + b * a.H + h) * a.parts + part;
-    part_store<L::DB>(acc, part_at<L::DB>(a.part, at, wave), lane);
-    float* ml = a.ml + (at * 4 + wave) * 64;
+    const int64_t at = ((int64_t)(qw / 32) * BH + b * a.H + h) * a.parts + part;
+    part_store<L::DB>(acc, part_at<L::DB>(a.part, at), lane);
+    float* ml = a.ml + at * 64;
     if (g == 0) {
       ml[l32] = m_run;
       ml[32 + l32] = l;
@@ -324,49 +348,64 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a) {
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int BH = a.B * a.H, qt = blockIdx.x / BH, bh = blockIdx.x % BH, qw = qt * 128 + 32 * wave;
   if (qw >= a.Sq) return;
-  const int64_t at = (int64_t)blockIdx.x * a.parts;
+  const int64_t at = ((int64_t)(qw / 32) * BH + bh) * a.parts;
   float m = -INFINITY;
-  for (int i = 0; i < a.parts; ++i) m = fmaxf(m, a.ml[((at + i) * 4 + wave) * 64 + l32]);
+  for (int i = 0; i < a.parts; ++i) m = fmaxf(m, a.ml[(at + i) * 64 + l32]);
   const float ref = m == -INFINITY ? 0.f : m;
   f32x16 acc[L::DB];
 #pragma unroll
   for (int i = 0; i < L::DB; ++i) acc[i] = f32x16{};
   float l = 0.f;
   for (int i = 0; i < a.parts; ++i) {
-    const float* ml = a.ml + ((at + i) * 4 + wave) * 64;
+    const float* ml = a.ml + (at + i) * 64;
     const float w = fast_exp2(ml[l32] - ref);
     l = __builtin_fmaf(ml[32 + l32], w, l);
-    part_add<L::DB>(acc, part_at<L::DB>(a.part, at + i, wave), lane, w);
+    part_add<L::DB>(acc, part_at<L::DB>(a.part, at + i), lane, w);
   }
   finish_rows<E, D>(a, bh / a.H, bh % a.H, qw, acc, m, l, stage[wave]);
 }
 
+int64_t tiles128(const SAttnArgs& a) { return (int64_t)((a.Sq + 127) / 128) * a.B * a.H; }
+
+// Whether two waves share a query row's keys: while workgroups are few, shorter steps
+// and twice the workgroups (as attn_fwd.hip's key_split).
+bool key_split(const SAttnArgs& a) {
+  return tiles128(a) <= (!a.causal ? 128 : a.D > 64 ? 256 : 512);
+}
+
 // Parts a query tile's keys are split into.  A workgroup is a serial chain of key
 // tiles, and a launch of few of them leaves the chip empty; a split costs writing
-// and reading the parts' fp32 O once.  Up to one workgroup per CU, no fewer than
-// four key tiles to a part.
-int fwd_parts(const SAttnArgs& a) {
-  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H;
-  const int64_t most = (a.Sk + 255) / 256, want = 512 / n;
+// and reading the parts' fp32 O once.  Up to one workgroup per CU, two where chains
+// are 32 tiles or longer and the join matters less (B1 H4 S4096 D64: 29 us against
+// 42), three for fp32, whose products take sixteen times as long; no fewer than four
+// key tiles to a part.
+int fwd_parts(const SAttnArgs& a, bool f32) {
+  const int64_t n = tiles128(a) * (key_split(a) ? 2 : 1);
+  const int64_t most = (a.Sk + 255) / 256, want = (f32 ? 768 : a.Sk >= 2048 ? 512 : 256) / n;
   return (int)(want < 2 ? 1 : want < most ? want : most);
+}
+
+template <typename E, int D, int KS>
+hipError_t launch_k(const SAttnArgs& a, bool cap, hipStream_t st) {
+  const dim3 grid((a.Sq + 128 / KS - 1) / (128 / KS) * a.B * a.H * a.parts), block(256);
+  if (cap && a.slopes)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, true, KS>), grid, block, 0, st, a);
+  else if (cap)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, false, KS>), grid, block, 0, st, a);
+  else if (a.slopes)
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, true, KS>), grid, block, 0, st, a);
+  else
+    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, false, KS>), grid, block, 0, st, a);
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess || a.parts == 1) return e;
+  hipLaunchKernelGGL((sattn_join_kernel<E, D>), dim3((a.Sq + 127) / 128 * a.B * a.H), block, 0, st,
+                     a);
+  return hipGetLastError();
 }
 
 template <typename E, int D>
 hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
-  const int n = (a.Sq + 127) / 128 * a.B * a.H;
-  const dim3 grid(n * a.parts), block(256);
-  if (cap && a.slopes)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, true>), grid, block, 0, st, a);
-  else if (cap)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, false>), grid, block, 0, st, a);
-  else if (a.slopes)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, true>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, false>), grid, block, 0, st, a);
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.parts == 1) return e;
-  hipLaunchKernelGGL((sattn_join_kernel<E, D>), dim3(n), block, 0, st, a);
-  return hipGetLastError();
+  return key_split(a) ? launch_k<E, D, 2>(a, cap, st) : launch_k<E, D, 1>(a, cap, st);
 }
 
 template <typename E>
@@ -384,16 +423,13 @@ hipError_t launch_doc_tiles(const int* docs, void* tiles, int B, int Sq, int Sk,
   return hipGetLastError();
 }
 
-int64_t sattn_fwd_workspace(const SAttnArgs& a) {
-  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H, p = fwd_parts(a);
-  return p == 1 ? 0 : n * p * (128 * (a.D <= 64 ? 64 : 128) + 256);
-}
-
-void sattn_fwd_split(SAttnArgs& a, float* ws) {
-  const int64_t n = (int64_t)((a.Sq + 127) / 128) * a.B * a.H;
-  a.parts = fwd_parts(a);
+void sattn_fwd_split(int dtype, SAttnArgs& a, float* ws, int64_t* elems) {
+  const int64_t blocks = 4 * tiles128(a);  // of 32 rows
+  const int64_t per = 32 * (a.D <= 64 ? 64 : 128);
+  a.parts = fwd_parts(a, dtype == 0);
+  if (elems) *elems = a.parts > 1 ? blocks * a.parts * (per + 64) : 0;
   a.part = ws;
-  a.ml = ws + n * a.parts * (128 * (a.D <= 64 ? 64 : 128));
+  a.ml = ws + blocks * a.parts * per;
 }
 
 hipError_t launch_sattn_fwd(int dtype, const SAttnArgs& a, bool cap, hipStream_t st) {
