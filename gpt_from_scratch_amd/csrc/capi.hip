@@ -1445,10 +1445,11 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
 int64_t mi_sattn_fwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
   if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
   int64_t most = 0;
-  for (int causal = 0; causal < 2; ++causal) {  // the split depends on it
-    mi_score_mods mods = {};
-    mods.causal = causal;
-    mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, mods, nullptr);
+  for (int i = 0; i < 4; ++i) {  // the split depends on causal and on documents
+    mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr);
+    static const int none = 0;
+    a.causal = i & 1;
+    a.docs = i & 2 ? &none : nullptr;
     int64_t n = 0;
     mi::sattn_fwd_split(dtype, a, nullptr, &n);
     most = n > most ? n : most;
@@ -1458,10 +1459,16 @@ int64_t mi_sattn_fwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int
 
 int64_t mi_sattn_bwd_workspace(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D) {
   if (check_sattn(dtype, B, H, Hk, Sq, Sk, D, 1.f, 0.f) != MI_OK) return 0;
-  mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr);
-  int64_t n = 0;
-  mi::sattn_bwd_split(a, nullptr, &n);
-  return n;
+  int64_t most = 0;
+  for (int docs = 0; docs < 2; ++docs) {  // the split depends on there being any
+    mi::SAttnArgs a = sattn_args(dtype, B, H, Hk, Sq, Sk, D, 1.f, {}, nullptr);
+    static const int none = 0;
+    a.docs = docs ? &none : nullptr;
+    int64_t n = 0;
+    mi::sattn_bwd_split(a, nullptr, &n);
+    most = n > most ? n : most;
+  }
+  return most;
 }
 
 mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int D, float scale,

@@ -155,6 +155,10 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   // with a causal mask alone no visible key is ahead of its query
   const bool one_sided = BIAS && a.causal && !a.prefix;
   const float gstep = one_sided ? slope2 : 0.f;
+  // A wave in its P V products goes before one in its softmax, whose time the products
+  // hide: B2 H16/4 S4096 D128 155 -> 141 us, with a bias 173 -> 161.  With a cap the
+  // softmax is the longer part and must not wait (172 -> 182).
+  constexpr bool kPrio = !CAP;
 
   auto step = [&](int cur, int nxt, auto slot) __attribute__((always_inline)) {
     constexpr int I = decltype(slot)::value;
@@ -264,6 +268,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
         for (int ng = 0; ng < L::NG; ++ng) p[kb][ng] = Elem<E>::operand(s[kb], ng);
       }
       l_run += ps[0] + ps[1];
+      if constexpr (kPrio) __builtin_amdgcn_s_setprio(1);
 #pragma unroll
       for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -271,6 +276,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
 #pragma unroll
           for (int db = 0; db < L::DB; ++db)
             acc[db] = Elem<E>::mfma(rd.col(vt, kb, ng, db), p[kb][ng], acc[db]);
+      if constexpr (kPrio) __builtin_amdgcn_s_setprio(0);
     }
     __syncthreads();
   };
@@ -368,8 +374,12 @@ __global__ __launch_bounds__(256) void sattn_join_kernel(SAttnArgs a) {
 int64_t tiles128(const SAttnArgs& a) { return (int64_t)((a.Sq + 127) / 128) * a.B * a.H; }
 
 // Whether two waves share a query row's keys: while workgroups are few, shorter steps
-// and twice the workgroups (as attn_fwd.hip's key_split).
+// and twice the workgroups (as attn_fwd.hip's key_split).  Documents leave short
+// chains of different lengths, and at D <= 64 the split evens them out up to twice as
+// many (us whole / split, 768 and 1024 tiles: 29.1 / 24.9, 43.6 / 37.0; at D = 128,
+// 1024 tiles: 57 / 70, 82 / 85).
 bool key_split(const SAttnArgs& a) {
+  if (a.docs && a.D <= 64) return tiles128(a) <= 1024;
   return tiles128(a) <= (!a.causal ? 128 : a.D > 64 ? 256 : 512);
 }
 
