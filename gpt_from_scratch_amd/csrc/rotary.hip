@@ -11,11 +11,17 @@
 //     dx = r (g - n^ mean(g n^)),   dw = sum over rows of d n^
 //   r is recomputed from x, which the backward reads anyway.
 //
-// Bound by reading and writing q and k once (twice read in the norm's backward).
-// A group of LPR lanes holds a row, two 16-byte chunks per lane: adjacent ones
-// for adjacent pairs, chunks R / 2 apart for halves, so that a pair lies in one
-// lane either way and its angles are the same consecutive ones.  A group takes U
-// heads of one token with one load of the angles and with all rows in flight.
+// Bound by reading and writing q and k once (x read again in the norm's backward).
+// A group of LPR lanes holds a row, two 16-byte chunks per lane, R / 2 elements
+// apart, so that a pair lies in one lane in either layout and a group's loads are
+// contiguous.  A group takes U heads of one token with one load of the angles and
+// with all rows in flight; they are spaced so that the groups of a wave take
+// neighbouring heads at each step.  With U consecutive heads and the chunks of
+// adjacent pairs side by side, the rotation below took 42 us, the norm 15 us.
+//   rotation, bf16 B4 S2048 H32/8 D128 R64: 35.4 us, 4.7 TB/s (a copy: 5.1); U = 4 37, 1 34.4
+//   rotation, fp32 B3 S1000 H12 D64:         7.7 us (U = 4: 8.7, 1: 9.2)
+//   norm, fp16 B4 S4096 H32/8 D128: forward 65 us (U = 2: 64, 1: 70), backward 95 us
+//   norm, bf16 B8 S1024 H12 D64: forward 11 us (U = 2: 14, 1: 13), backward 22 + 3.6 us
 #include "mi_device.h"
 #include "mi_kernels.h"
 
@@ -63,6 +69,11 @@ __device__ __forceinline__ float load_as(int dt, const void* p, int64_t i) {
 template <int N>
 __device__ __forceinline__ void load_values(int dt, const void* p, int64_t i, float* f) {
   if (dt == 0) {
+    if constexpr (N == 2) {
+      const u32x2 w = *(const u32x2*)((const float*)p + i);
+      f[0] = __uint_as_float(w[0]);
+      f[1] = __uint_as_float(w[1]);
+    }
 #pragma unroll
     for (int k = 0; k < N / 4; ++k) {
       const f32x4 w = *(const f32x4*)((const float*)p + i + 4 * k);
@@ -75,10 +86,12 @@ __device__ __forceinline__ void load_values(int dt, const void* p, int64_t i, fl
       const u32x4 x = *(const u32x4*)((const uint16_t*)p + i);
 #pragma unroll
       for (int k = 0; k < 4; ++k) w[k] = x[k];
-    } else {
+    } else if constexpr (N == 4) {
       const u32x2 x = *(const u32x2*)((const uint16_t*)p + i);
       w[0] = x[0];
       w[1] = x[1];
+    } else {
+      w[0] = *(const uint32_t*)((const uint16_t*)p + i);
     }
 #pragma unroll
     for (int k = 0; k < N / 2; ++k) {
@@ -140,14 +153,33 @@ struct Chunks {
 };
 template <int N>
 __device__ __forceinline__ Chunks chunks(const RotaryArgs& a, int l) {
-  const int half = a.R / (2 * N);  // lanes with pairs
+  const int half = a.R / (2 * N), lanes = a.D / (2 * N);  // lanes with pairs, all lanes
   Chunks c;
-  c.have = l < a.D / (2 * N);
+  c.have = l < lanes;
   c.turned = l < half;
-  const bool split = c.turned && !a.interleaved;
-  c.c0 = split ? l : 2 * l;
-  c.c1 = split ? l + half : 2 * l + 1;
+  c.c0 = c.turned ? l : l + half;
+  c.c1 = c.turned ? l + half : l + lanes;
   return c;
+}
+
+// The angles of a lane's pairs at position p (NaN where the tables end).
+template <int N>
+__device__ __forceinline__ void load_angles(const RotaryArgs& a, const Chunks& c, int64_t p,
+                                            float (&cs)[N], float (&sn)[N]) {
+  const int64_t row = p < 0 ? 0 : p;
+  if (a.interleaved) {
+    load_values<N / 2>(a.tab_dt, a.cos, row * a.cs_s + c.c0 * (N / 2), cs);
+    load_values<N / 2>(a.tab_dt, a.cos, row * a.cs_s + c.c1 * (N / 2), cs + N / 2);
+    load_values<N / 2>(a.tab_dt, a.sin, row * a.ss_s + c.c0 * (N / 2), sn);
+    load_values<N / 2>(a.tab_dt, a.sin, row * a.ss_s + c.c1 * (N / 2), sn + N / 2);
+  } else {
+    load_values<N>(a.tab_dt, a.cos, row * a.cs_s + c.c0 * N, cs);
+    load_values<N>(a.tab_dt, a.sin, row * a.ss_s + c.c0 * N, sn);
+  }
+  if (p < 0) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) cs[i] = sn[i] = __builtin_nanf("");
+  }
 }
 
 template <int DT, int LPR, int MODE, int U>
@@ -160,11 +192,12 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryArgs a, FastDiv d
   const Chunks c = chunks<N>(a, threadIdx.x % LPR);
   // item = token * (head blocks of q and k) + head block
   const uint32_t sb = fdiv(item, dhb);
-  int h0 = (int)(item - sb * dhb.d) * U;
-  const int qh = (a.t[0].heads + U - 1) / U * U;
-  const bool second = h0 >= qh;
-  if (second) h0 -= qh;
+  int h0 = (int)(item - sb * dhb.d);
+  const int qhb = (a.t[0].heads + U - 1) / U;
+  const bool second = h0 >= qhb;
+  if (second) h0 -= qhb;
   const RotaryTensor& t = a.t[second];
+  const int dh = second ? (int)dhb.d - qhb : qhb;  // heads h0, h0 + dh, ...
   const uint32_t s = fdiv(sb, dB), b = sb - s * dB.d;
   const T* x = (const T*)t.x + s * t.x_ss + b * t.x_sb;
   T* out = (T*)t.out + s * t.o_ss + b * t.o_sb;
@@ -173,22 +206,13 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryArgs a, FastDiv d
 #pragma unroll
   for (int u = 0; u < U; ++u) {
     w[u][0] = w[u][1] = u32x4{0, 0, 0, 0};
-    if (c.have && h0 + u < t.heads) {
-      w[u][0] = __builtin_nontemporal_load((const u32x4*)(x + (h0 + u) * t.x_sh) + c.c0);
-      w[u][1] = __builtin_nontemporal_load((const u32x4*)(x + (h0 + u) * t.x_sh) + c.c1);
+    if (c.have && h0 + u * dh < t.heads) {
+      w[u][0] = __builtin_nontemporal_load((const u32x4*)(x + (h0 + u * dh) * t.x_sh) + c.c0);
+      w[u][1] = __builtin_nontemporal_load((const u32x4*)(x + (h0 + u * dh) * t.x_sh) + c.c1);
     }
   }
   float cs[N], sn[N];
-  if (c.turned) {
-    const int64_t p = position(a, s, b);
-    const int l = threadIdx.x % LPR;
-    load_values<N>(a.tab_dt, a.cos, (p < 0 ? 0 : p) * a.cs_s + l * N, cs);
-    load_values<N>(a.tab_dt, a.sin, (p < 0 ? 0 : p) * a.ss_s + l * N, sn);
-    if (p < 0) {
-#pragma unroll
-      for (int i = 0; i < N; ++i) cs[i] = sn[i] = __builtin_nanf("");
-    }
-  }
+  if (c.turned) load_angles<N>(a, c, position(a, s, b), cs, sn);
   float nw[2 * N];
   if (MODE == kNorm && c.have) {
     load_values<N>(a.w_dt, t.w, c.c0 * N, nw);
@@ -210,10 +234,10 @@ __global__ __launch_bounds__(256) void rotary_vec_kernel(RotaryArgs a, FastDiv d
         for (int i = 0; i < 2 * N; ++i) f[i] = f[i] * r * nw[i];
       }
     }
-    if (!c.have || h0 + u >= t.heads) continue;
+    if (!c.have || h0 + u * dh >= t.heads) continue;
     if (c.turned) turn<DT, N>(f, cs, sn, a.interleaved, MODE == kRotate && a.inverse);
-    __builtin_nontemporal_store(Vec<DT>::pack(f), (u32x4*)(out + (h0 + u) * t.o_sh) + c.c0);
-    __builtin_nontemporal_store(Vec<DT>::pack(f + N), (u32x4*)(out + (h0 + u) * t.o_sh) + c.c1);
+    __builtin_nontemporal_store(Vec<DT>::pack(f), (u32x4*)(out + (h0 + u * dh) * t.o_sh) + c.c0);
+    __builtin_nontemporal_store(Vec<DT>::pack(f + N), (u32x4*)(out + (h0 + u * dh) * t.o_sh) + c.c1);
   }
 }
 
@@ -241,7 +265,7 @@ __global__ __launch_bounds__(256) void rotary_grad_vec_kernel(RotaryArgs a, Fast
   for (uint32_t item = first * GROUPS + threadIdx.x / LPR; item < items;
        item += a.blocks[second] * GROUPS) {
     const uint32_t sb = item / nhb;
-    const int h0 = (item - sb * nhb) * U;
+    const int h0 = item - sb * nhb;
     const uint32_t s = fdiv(sb, dB), b = sb - s * dB.d;
     const T* x = (const T*)t.x + s * t.x_ss + b * t.x_sb;
     const T* dy = (const T*)t.dy + s * t.dy_ss + b * t.dy_sb;
@@ -250,8 +274,8 @@ __global__ __launch_bounds__(256) void rotary_grad_vec_kernel(RotaryArgs a, Fast
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       xw[u][0] = xw[u][1] = dyw[u][0] = dyw[u][1] = u32x4{0, 0, 0, 0};
-      if (c.have && h0 + u < t.heads) {
-        const int h = h0 + u;
+      if (c.have && h0 + u * (int)nhb < t.heads) {
+        const int h = h0 + u * (int)nhb;
         xw[u][0] = __builtin_nontemporal_load((const u32x4*)(x + h * t.x_sh) + c.c0);
         xw[u][1] = __builtin_nontemporal_load((const u32x4*)(x + h * t.x_sh) + c.c1);
         dyw[u][0] = __builtin_nontemporal_load((const u32x4*)(dy + h * t.dy_sh) + c.c0);
@@ -259,15 +283,7 @@ __global__ __launch_bounds__(256) void rotary_grad_vec_kernel(RotaryArgs a, Fast
       }
     }
     float cs[N], sn[N];
-    if (c.turned) {
-      const int64_t p = position(a, s, b);
-      load_values<N>(a.tab_dt, a.cos, (p < 0 ? 0 : p) * a.cs_s + l * N, cs);
-      load_values<N>(a.tab_dt, a.sin, (p < 0 ? 0 : p) * a.ss_s + l * N, sn);
-      if (p < 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) cs[i] = sn[i] = __builtin_nanf("");
-      }
-    }
+    if (c.turned) load_angles<N>(a, c, position(a, s, b), cs, sn);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       float f[2 * N], d[2 * N];
@@ -284,7 +300,7 @@ __global__ __launch_bounds__(256) void rotary_grad_vec_kernel(RotaryArgs a, Fast
       }
       const float r = rsqrtf(row_sum<LPR>(q) * inv_d + a.eps);
       const float m = row_sum<LPR>(gn) * r * inv_d;  // mean(g n^)
-      if (h0 + u >= t.heads) continue;
+      if (h0 + u * (int)nhb >= t.heads) continue;
 #pragma unroll
       for (int i = 0; i < 2 * N; ++i) {
         const float n = f[i] * r;
@@ -292,8 +308,8 @@ __global__ __launch_bounds__(256) void rotary_grad_vec_kernel(RotaryArgs a, Fast
         f[i] = r * (d[i] * nw[i] - n * m);
       }
       if (!c.have) continue;
-      __builtin_nontemporal_store(Vec<DT>::pack(f), (u32x4*)(out + (h0 + u) * t.o_sh) + c.c0);
-      __builtin_nontemporal_store(Vec<DT>::pack(f + N), (u32x4*)(out + (h0 + u) * t.o_sh) + c.c1);
+      __builtin_nontemporal_store(Vec<DT>::pack(f), (u32x4*)(out + (h0 + u * (int)nhb) * t.o_sh) + c.c0);
+      __builtin_nontemporal_store(Vec<DT>::pack(f + N), (u32x4*)(out + (h0 + u * (int)nhb) * t.o_sh) + c.c1);
     }
   }
   // groups of the wave, then the four waves
@@ -432,8 +448,10 @@ __global__ __launch_bounds__(1024) void rotary_dw_kernel(RotaryArgs a) {
   const int col = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
   const int first = blockIdx.y ? a.blocks[0] : 0, n = a.blocks[blockIdx.y];
   float v = 0.f;
-  if (col < a.D)
+  if (col < a.D) {
+#pragma unroll 8
     for (int i = lane; i < n; i += 32) v += a.part[(int64_t)(first + i) * a.D + col];
+  }
   sum[lane][threadIdx.x % 32] = v;
   __syncthreads();
   if (lane == 0 && col < a.D) {
@@ -452,15 +470,16 @@ hipError_t launch_vec(int mode, const RotaryArgs& a, hipStream_t st) {
     hipLaunchKernelGGL((rotary_grad_vec_kernel<DT, LPR, 2>), dim3(a.blocks[0] + a.blocks[1]),
                        dim3(256), 0, st, a, dB);
   } else {
-    constexpr int U = 4;
-    const uint32_t hb = (a.t[0].heads + U - 1) / U + (a.t[1].heads + U - 1) / U;
+    constexpr int UR = 2, U = 4;
+    const int u = mode == kNorm ? U : UR;
+    const uint32_t hb = (a.t[0].heads + u - 1) / u + (a.t[1].heads + u - 1) / u;
     const uint32_t items = (uint32_t)a.S * a.B * hb;
     const dim3 grid((items + 256 / LPR - 1) / (256 / LPR)), block(256);
     if (mode == kNorm)
       hipLaunchKernelGGL((rotary_vec_kernel<DT, LPR, kNorm, U>), grid, block, 0, st, a,
                          make_fastdiv(hb), dB, items);
     else
-      hipLaunchKernelGGL((rotary_vec_kernel<DT, LPR, kRotate, U>), grid, block, 0, st, a,
+      hipLaunchKernelGGL((rotary_vec_kernel<DT, LPR, kRotate, UR>), grid, block, 0, st, a,
                          make_fastdiv(hb), dB, items);
   }
   return hipGetLastError();
