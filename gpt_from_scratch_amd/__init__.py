@@ -15,14 +15,14 @@ from .mlp import ParallelMLP, SwiGLU, swiglu
 from .normalization import FusedAddRMSNorm, FusedRMSNorm, RMSNorm, add_rms_norm, rms_norm
 from .optimizer import DistributedOptimizer
 from .flash_attn import FlashAttn, apply_flash_attn, flash_attn_backward, flash_attn_forward
-from .position_embeddings import RotaryEmbedding
+from .position_embeddings import RotaryEmbedding, RotaryScaling
 from .rope import RoPE, RoPEQK, TritonRoPE, apply_rope, apply_rope_qk
 from .rotary import QKNormRotary, RotaryQK, apply_rotary_qk, qk_norm_rotary
 from .scored_attn import ScoredAttn, decode_attn, scored_attn, scored_attn_forward
 
 __all__ = [
     "FlashAttn", "apply_flash_attn", "flash_attn_forward", "flash_attn_backward",
-    "RotaryEmbedding", "RoPE", "RoPEQK", "TritonRoPE", "apply_rope", "apply_rope_qk",
+    "RotaryEmbedding", "RotaryScaling", "RoPE", "RoPEQK", "TritonRoPE", "apply_rope", "apply_rope_qk",
     "AttentionBlock", "attention_block",
     "VocabParallelCrossEntropy", "_VocabParallelCrossEntropy", "vocab_parallel_cross_entropy",
     "RMSNorm", "FusedRMSNorm", "rms_norm", "FusedAddRMSNorm", "add_rms_norm", "SwiGLU", "swiglu", "ParallelMLP",

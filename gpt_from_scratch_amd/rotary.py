@@ -15,7 +15,8 @@ first ``2 * cos.shape[1]`` elements of each head of q ``[S, B, H, D]`` and k
 head, ``n = x * rsqrt(mean(x^2) + eps) * weight`` over its D elements, then turns n:
 one pass over q and k forward, one backward (and the sum of the weights'
 gradients).  Both compute in fp32 and round once.  Tables for long contexts come
-from ``RotaryEmbedding(..., scaling=...)``.
+from ``RotaryEmbedding(..., scaling=RotaryScaling(...))``; ``RotaryEmbedding(2 * n)``
+gives those of a part of the head.
 
 The reference has the interleaved rotation of whole heads at positions
 ``0 .. S - 1`` (core/rope_triton.py:10-148).
