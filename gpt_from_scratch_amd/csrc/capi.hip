@@ -1336,8 +1336,9 @@ mi_status check_sattn(int dtype, int B, int H, int Hk, int Sq, int Sk, int D, fl
     return fail(MI_ERR_UNSUPPORTED, "sequence too long for one launch");
   if (!(scale > 0.f) || std::isinf(scale))
     return fail(MI_ERR_INVALID_ARGUMENT, "scale must be a positive finite number");
-  if (!(softcap >= 0.f) || std::isinf(softcap))
-    return fail(MI_ERR_INVALID_ARGUMENT, "softcap must be finite and positive, or 0 for none");
+  // the 16-bit types' form of the capped score is off by softcap * 2^-23
+  if (!(softcap >= 0.99e-6f && softcap <= 1e4f) && softcap != 0.f)
+    return fail(MI_ERR_INVALID_ARGUMENT, "softcap must be between 1e-6 and 1e4, or 0 for none");
   return MI_OK;
 }
 
@@ -1430,7 +1431,8 @@ mi_status mi_sattn_fwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
   a.o = targ(o, o_strides);
   a.olo = o_lo;
   a.lse = lse;
-  if (((uintptr_t)o_lo) % 16) return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-byte aligned rows wanted");
+  if (o_lo && (dtype == MI_F32 || ((uintptr_t)o_lo) % 16))
+    return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-bit types and 16-byte aligned rows only");
   int64_t want = 0;
   mi::sattn_fwd_split(dtype, a, workspace, &want);
   if ((st = check_workspace(workspace, workspace_elems, want)) != MI_OK) return st;
@@ -1488,7 +1490,8 @@ mi_status mi_sattn_bwd(mi_dtype dtype, int B, int H, int Hk, int Sq, int Sk, int
                                  {dv, dv_strides}})) != MI_OK)
     return st;
   if (lse == nullptr) return fail(MI_ERR_INVALID_ARGUMENT, "lse: null pointer");
-  if (((uintptr_t)o_lo) % 16) return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-byte aligned rows wanted");
+  if (o_lo && (dtype == MI_F32 || ((uintptr_t)o_lo) % 16))
+    return fail(MI_ERR_UNSUPPORTED, "o_lo: 16-bit types and 16-byte aligned rows only");
   if ((st = check_workspace(workspace, workspace_elems,
                             mi_sattn_bwd_workspace(dtype, B, H, Hk, Sq, Sk, D))) != MI_OK)
     return st;

@@ -1148,7 +1148,7 @@ PyObject* py_qk_norm_rotary(PyObject*, Args a, Py_ssize_t n) {
 bool cap_and_scale(PyObject* cap, PyObject* scale, int64_t D, Mods& m) {
   m.cap = 0.0;
   m.scale = 1.0 / std::sqrt((double)D);
-  return (cap == Py_None || (number(cap, m.cap) && m.cap > 0.0)) &&
+  return (cap == Py_None || (number(cap, m.cap) && m.cap >= 1e-6 && m.cap <= 1e4)) &&
          (scale == Py_None || number(scale, m.scale));
 }
 

@@ -54,16 +54,19 @@ def _check_heads(q, k, v, q_dims, what):
 
 
 def _check_scores(q, softcap, slopes, scale):
-    if softcap is not None and not (softcap > 0 and math.isfinite(softcap)):
-        raise ValueError(f"softcap must be positive and finite (or None), got {softcap}")
+    if softcap is not None and not 1e-6 <= softcap <= 1e4:
+        raise ValueError(f"softcap must be between 1e-6 and 1e4 (or None), got {softcap}")
     if not (scale > 0 and math.isfinite(scale)):
         raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
     if slopes is not None:
         if slopes.dtype != torch.float32 or tuple(slopes.shape) != (q.shape[1],):
             raise ValueError(f"slopes must be float32 [{q.shape[1]}]; got {slopes.dtype} "
                              f"{tuple(slopes.shape)}")
-        if slopes.requires_grad and torch.is_grad_enabled():
-            raise ValueError("slopes take no gradient: detach them")
+
+
+def _check_slopes_grad(slopes):
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes take no gradient: detach them")
 
 
 def _check_ints(name, t, shape):
@@ -140,6 +143,7 @@ def scored_attn(q, k, v, causal: bool = True, softcap=None, slopes=None, documen
                                softmax_scale)
     if o is not None:
         return o
+    _check_slopes_grad(slopes)
     return ScoredAttn.apply(q, k, v, causal, softcap, slopes, document_ids, prefix_lens,
                             _scale(q, softmax_scale))
 
@@ -166,6 +170,7 @@ def decode_attn(q, k, v, lengths=None, softcap=None, slopes=None, softmax_scale=
     scale = _scale(q, softmax_scale)
     _check_heads(q, k, v, 3, "q must be [B, H, D] and k, v [B, Hk, S, D]")
     _check_scores(q, softcap, slopes, scale)
+    _check_slopes_grad(slopes)
     _check_ints("lengths", lengths, (q.shape[0],))
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v)):
         raise RuntimeError("decode_attn has no backward: call it under torch.no_grad(), or use "

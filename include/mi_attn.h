@@ -556,7 +556,7 @@ mi_status mi_qk_norm_rotary_bwd(mi_dtype dtype, mi_dtype w_dtype, const mi_rotar
  */
 typedef struct mi_score_mods {
   int causal;
-  float softcap;               /* 0: none */
+  float softcap;               /* 1e-6 .. 1e4, or 0: none */
   const float* slopes;         /* [H] or NULL */
   const int32_t* document_ids; /* [B, Sk] dense or NULL */
   const int32_t* prefix_lens;  /* [B] or NULL; with causal only */
