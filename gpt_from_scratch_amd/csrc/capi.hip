@@ -1188,7 +1188,9 @@ mi::RotaryArgs rotary_args(mi_dtype dtype, const mi_rotary& h, const void* const
   const int esz = elem_size(dtype), n = 16 / esz;
   // a lane's n angles come with aligned loads: 16 bytes, or all n of them if less
   const int tsz = elem_size(h.tab_dtype), ab = n * tsz < 16 ? n * tsz : 16;
-  vec = mi::rotary_vec_ok(dtype, h.D, h.R) && a.cs_i == 1 && a.ss_i == 1 &&
+  // (a launch has at most 2^32 threads, and a group at most 8 lanes for every 16 elements)
+  vec = mi::rotary_vec_ok(dtype, h.D, h.R) &&
+        (double)h.S * h.B * ((double)h.H + h.Hk) * h.D < 8589934592.0 && a.cs_i == 1 && a.ss_i == 1 &&
         a.cs_s * tsz % ab == 0 && a.ss_s * tsz % ab == 0 && ((uintptr_t)a.cos) % ab == 0 &&
         ((uintptr_t)a.sin) % ab == 0;
   for (int i = 0; i < 2; ++i) {
@@ -1331,8 +1333,10 @@ mi_status check_sattn(int dtype, int B, int H, int Hk, int Sq, int Sk, int D, fl
   if (Sq > Sk) return fail(MI_ERR_INVALID_ARGUMENT, "more queries (%d) than keys (%d)", Sq, Sk);
   if (D % 8 || D > 128)
     return fail(MI_ERR_UNSUPPORTED, "head dim %d: a multiple of 8 up to 128", D);
-  // tile indexes and positions (as exact floats) keep 24 bits, rows 31
-  if (Sk > (1 << 24) || (double)B * H * Sq >= 2147483648.0 || (double)B * Hk * Sk >= 2147483648.0)
+  // tile indexes and positions (as exact floats) keep 24 bits, a launch 2^32 threads
+  // (2^24 workgroups of 256, each with at least 64 rows)
+  if (Sk > (1 << 24) || (double)B * H * ((Sq + 63) / 64) >= 16777216.0 ||
+      (double)B * Hk * ((Sk + 63) / 64) >= 16777216.0)
     return fail(MI_ERR_UNSUPPORTED, "sequence too long for one launch");
   if (!(scale > 0.f) || std::isinf(scale))
     return fail(MI_ERR_INVALID_ARGUMENT, "scale must be a positive finite number");

@@ -495,7 +495,8 @@ hipError_t launch_t(int mode, const RotaryArgs& a, bool vec, hipStream_t st) {
     return launch_vec<DT, 32>(mode, a, st);
   }
   const uint32_t rows = (uint32_t)a.S * a.B * (a.t[0].heads + a.t[1].heads);
-  const dim3 grid((rows + 3) / 4), block(256);
+  const uint32_t wgs = rows / 4 + 1;  // they loop; a launch has at most 2^32 threads
+  const dim3 grid(wgs < (1u << 22) ? wgs : 1u << 22), block(256);
   if (mode == kRotate)
     hipLaunchKernelGGL((rotary_any_kernel<DT, kRotate>), grid, block, 0, st, a, rows);
   else if (mode == kNorm)

@@ -143,7 +143,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   const int k0 = kt * OWN, kw = k0 + 32 * wave, krow = kw + l32;
   const bool wave_valid = kw < Sk;
   const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
-  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
   const int kdoc = docs && krow < Sk ? docs[krow] : 0;
   // first query position that sees this lane's key, and the wave's first
   int qfirst = 0, wfirst = 0;
@@ -384,7 +384,7 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   const int q0 = qt * OWN, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
   const bool wave_valid = qw < Sq;
   const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
-  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
   const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
   const int qdoc = docs && qrow < Sq ? docs[qpos] : 0;
   int klast = Sk - 1, wlast = Sk - 1;

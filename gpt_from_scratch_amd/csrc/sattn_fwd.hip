@@ -95,7 +95,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   const int slice = KS == 1 ? 0 : wave & 1;
   const bool wave_valid = qw < Sq;
   const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
-  const int prefix = a.prefix ? a.prefix[b] : 0;
+  const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
   const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
 
   const char* qp = (const char*)a.q.ptr + (b * a.q.sb + h * a.q.sh + qrow * a.q.ss) * L::ESZ;

@@ -177,3 +177,29 @@ def test_gradients_of_some_inputs(gpu):
     assert all(torch.equal(s, t) for s, t in zip(got, dense))
     turned = torch.autograd.grad(o, x, do.transpose(1, 2).contiguous().transpose(1, 2))
     assert all(torch.equal(s, t) for s, t in zip(turned, want))
+
+
+def test_prefixes_of_any_value(gpu):
+    """Negative ones are none, ones past the end are all keys."""
+    from gpt_from_scratch_amd import scored_attn
+    x, do, _, _ = _attn_inputs(gpu, torch.bfloat16)
+    x = [torch.cat((t, t)).detach().requires_grad_() for t in x]
+    do = torch.cat((do, do))
+    pre = torch.tensor([-2 ** 31, -1, 2 ** 31 - 1, 200], dtype=torch.int32, device=gpu)
+    o = scored_attn(*x, prefix_lens=pre)
+    want = ref.attention(*(t.detach() for t in x), do, prefix=pre)
+    for n, g in zip(("o", "dq", "dk", "dv"), (o, *torch.autograd.grad(o, x, do))):
+        ref.within(n, g, want[n])
+
+
+def test_more_rows_than_one_wave_each(gpu):
+    """Heads of 4 elements, which no 16-byte chunk holds: 7e7 rows, past 2^32 threads."""
+    from gpt_from_scratch_amd import apply_rotary_qk
+    S, H = 1 << 21, 31
+    q, k = (randn((8, 1, n, 4), n, torch.float32, gpu).repeat(S // 8, 1, 1, 1) for n in (H, 2))
+    a = torch.rand(8, 2, generator=torch.Generator().manual_seed(1)).to(gpu).repeat(S // 8, 1)
+    cos, sin = a.cos(), a.sin()
+    for x, y in zip((q, k), apply_rotary_qk(q, k, cos, sin)):
+        first = ref.rotary(x[:8], cos[:8], sin[:8], None, True)
+        ref.within("first", y[:8], first)
+        assert torch.equal(y, y[:8].repeat(S // 8, 1, 1, 1))

@@ -222,6 +222,8 @@ NAN, INF = float("nan"), float("inf")
     (dict(sizes=(1, 2, 2, 64, 64, 136)), UNSUPPORTED),
     (dict(sizes=(1, 1, 1, 1, (1 << 24) + 1, 64)), UNSUPPORTED),
     (dict(sizes=(1 << 16, 1 << 15, 1, 1, 1, 64)), UNSUPPORTED),
+    (dict(sizes=(1 << 12, 1 << 12, 1, 1, 1, 64)), UNSUPPORTED),  # 2^32 threads
+    (dict(sizes=(1 << 10, 1 << 10, 1 << 10, 1, 1 << 10, 8)), UNSUPPORTED),
     (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=NAN), BAD), (dict(scale=INF), BAD),
     (dict(mods=_lib.ScoreMods(1, -1.0)), BAD), (dict(mods=_lib.ScoreMods(1, NAN)), BAD),
     (dict(mods=_lib.ScoreMods(1, INF)), BAD), (dict(mods=_lib.ScoreMods(1, 2e4)), BAD),
