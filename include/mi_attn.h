@@ -4,7 +4,8 @@
  * Causal / non-causal flash attention (forward with saved log-sum-exp, backward
  * producing dQ, dK, dV) and the interleaved-pair rotary position embedding, plus
  * the train step's fused vocabulary cross entropy, RMSNorm, SwiGLU and AdamW
- * step.
+ * step; and, beyond the reference, rotary embedding at given positions with the
+ * norm of each head, attention with modified scores, and its single-token form.
  * Every entry point takes plain device pointers, element strides and sizes, and
  * enqueues its kernels on the given HIP stream (a `hipStream_t`, passed as
  * `void*`; NULL means the null stream).  Nothing here allocates, frees or
