@@ -63,21 +63,23 @@ __device__ __forceinline__ bool lse_ramp(const SAttnArgs& a) {
 // ---------------------------------------------------------------------------
 // delta, and lse * log2(e) less the scores' constant
 // ---------------------------------------------------------------------------
-// Eight lanes per row of 16-byte chunks, four rows per lane with all their loads in
-// flight: 10 us at B8 H12 S1024 D64 (38 MB), 18 us at B2 H16 S4096 D128 (101 MB, 5.6 TB/s).
+// Eight lanes per row, R rows per lane with all their loads in flight (us for R = 1, 2, 4:
+// B8 H12 S1024 D64 9.1, 8.4, 9.4 for 38 MB; B2 H16 S4096 D128 16.5, 17.2, 17.9 for 101 MB;
+// fp32 B2 H12 S1000 D64 4.2, 4.6, 5.0).
 // Where no visible key is ahead of its query, and to the 16-bit types, which can
 // afford its rounding, the distance bias's part of the row's place in its block of 32
 // goes into lse2 here, once per row instead of once per score of dK / dV.
-template <typename E>
-__global__ __launch_bounds__(256) void sattn_delta_kernel(SAttnArgs a, uint32_t rows) {
-  constexpr int ESZ = Elem<E>::kBytes, R = 4, NC = 128 * ESZ / 16 / 8;
+template <typename E, int D, int R>
+__global__ __launch_bounds__(256) void sattn_delta_kernel(SAttnArgs a, uint32_t rows, FastDiv dS,
+                                                          FastDiv dH) {
+  constexpr int ESZ = Elem<E>::kBytes, NC = D * ESZ / 16 / 8;
   const int sub = threadIdx.x % 8;
   u32x4 x[R][NC], y[R][NC], z[R][NC];
   float ramp[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const uint32_t row = blockIdx.x * (32u * R) + 32 * i + threadIdx.x / 8;
-    const uint32_t bh = row / a.Sq, s = row - bh * a.Sq, b = bh / a.H, h = bh - b * a.H;
+    const uint32_t bh = fdiv(row, dS), s = row - bh * dS.d, b = fdiv(bh, dH), h = bh - b * dH.d;
     const int64_t at = (b * a.o.sb + h * a.o.sh + s * a.o.ss) * ESZ;
     const u32x4* o = (const u32x4*)((const char*)a.o.ptr + at);
     const u32x4* lo = a.olo ? (const u32x4*)((const char*)a.olo + at) : nullptr;
@@ -624,10 +626,12 @@ hipError_t launch_cb(const SAttnArgs& a, hipStream_t st) {
   return hipGetLastError();
 }
 
-template <typename E>
+template <typename E, int D>
 hipError_t launch_delta(const SAttnArgs& a, hipStream_t st) {
+  constexpr int R = D * Elem<E>::kBytes == 128 ? 2 : 1;
   const uint32_t rows = (uint32_t)a.B * a.H * a.Sq;
-  hipLaunchKernelGGL((sattn_delta_kernel<E>), dim3((rows + 127) / 128), dim3(256), 0, st, a, rows);
+  hipLaunchKernelGGL((sattn_delta_kernel<E, D, R>), dim3((rows + 32 * R - 1) / (32 * R)), dim3(256), 0,
+                     st, a, rows, make_fastdiv(a.Sq), make_fastdiv(a.H));
   return hipGetLastError();
 }
 
@@ -641,7 +645,7 @@ hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
 
 template <typename E>
 hipError_t launch_e(const SAttnArgs& a, bool cap, hipStream_t st) {
-  const hipError_t e = launch_delta<E>(a, st);
+  const hipError_t e = a.D <= 64 ? launch_delta<E, 64>(a, st) : launch_delta<E, 128>(a, st);
   if (e != hipSuccess) return e;
   return a.D <= 64 ? launch_d<E, 64>(a, cap, st) : launch_d<E, 128>(a, cap, st);
 }
