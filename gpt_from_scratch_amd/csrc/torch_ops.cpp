@@ -820,7 +820,7 @@ bool mods_ok(const Tensor& q, const Mods& m, int64_t B, int64_t H, int64_t Sk) {
 
 bool sattn_ok(const Tensor& q, const Tensor& k, const Tensor& v, const Mods& m) {
   return q.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes() && q.size(0) == k.size(0) &&
-         q.size(3) == k.size(3) && q.size(1) % k.size(1) == 0 && q.size(2) <= k.size(2) &&
+         k.numel() > 0 && q.size(3) == k.size(3) && q.size(1) % k.size(1) == 0 && q.size(2) <= k.size(2) &&
          code(q) >= 0 && q.scalar_type() == k.scalar_type() &&
          q.scalar_type() == v.scalar_type() && one_device(q, k, v) && q.size(3) % 8 == 0 &&
          q.size(3) <= 128 && k.size(2) <= 1 << 24 && q.size(0) < 1ll << 31 &&
@@ -1149,7 +1149,7 @@ bool cap_and_scale(PyObject* cap, PyObject* scale, int64_t D, Mods& m) {
   m.cap = 0.0;
   m.scale = 1.0 / std::sqrt((double)D);
   return (cap == Py_None || (number(cap, m.cap) && m.cap >= 1e-6 && m.cap <= 1e4)) &&
-         (scale == Py_None || number(scale, m.scale));
+         (scale == Py_None || (number(scale, m.scale) && m.scale > 0.0 && std::isfinite(m.scale)));
 }
 
 // q, k, v, causal, softcap, slopes, document_ids, prefix_lens, scale

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import scored_ref as ref
+import test_scored_checks as checks
 from test_gpu_scored_attn import documents, randn, run
 
 pytestmark = pytest.mark.gpu
@@ -203,3 +204,45 @@ def test_more_rows_than_one_wave_each(gpu):
         first = ref.rotary(x[:8], cos[:8], sin[:8], None, True)
         ref.within("first", y[:8], first)
         assert torch.equal(y, y[:8].repeat(S // 8, 1, 1, 1))
+
+
+def _moved(kw, device):
+    out = {n: t.detach().to(device).requires_grad_(t.requires_grad)
+           if isinstance(t, torch.Tensor) else t for n, t in kw.items()}
+    return out
+
+
+@pytest.mark.parametrize("kw,error,text", [c for c in checks.ROTARY if c[0]])
+def test_rotary_refuses_on_the_gpu(gpu, kw, error, text):
+    from gpt_from_scratch_amd import apply_rotary_qk, qk_norm_rotary
+    a = _moved(checks._rotary(**kw), gpu)
+    with pytest.raises(error, match=text):
+        apply_rotary_qk(**a)
+    w = torch.ones(a["q"].shape[-1], device=gpu)
+    with pytest.raises(error, match=text):
+        qk_norm_rotary(q_weight=w, k_weight=w, **a)
+
+
+@pytest.mark.parametrize("kw,error,text", [c for c in checks.ATTN + checks.MASKS if c[0]] + [
+    checks.SLOPES_GRAD, (dict(k=torch.zeros(2, 0, 32, 64), v=torch.zeros(2, 0, 32, 64)), ValueError,
+                         "no size 0")])
+def test_scored_attn_refuses_on_the_gpu(gpu, kw, error, text):
+    from gpt_from_scratch_amd import scored_attn, scored_attn_forward
+    a = _moved(checks._attn(**kw), gpu)
+    with pytest.raises(error, match=text):
+        scored_attn(**a)
+    if text != checks.SLOPES_GRAD[2]:
+        with pytest.raises(error, match=text):
+            scored_attn_forward(**a)
+
+
+@pytest.mark.parametrize("which", ["k", "v", "slopes", "document_ids", "prefix_lens"])
+def test_tensors_elsewhere_are_refused(gpu, which):
+    from gpt_from_scratch_amd import scored_attn
+    a = checks._attn(slopes=torch.zeros(4), document_ids=torch.zeros(2, 32, dtype=torch.int32),
+                     prefix_lens=torch.zeros(2, dtype=torch.int32))
+    b = _moved(a, gpu)
+    scored_attn(**b)
+    b[which] = a[which]
+    with pytest.raises(RuntimeError):
+        scored_attn(**b)
