@@ -246,3 +246,73 @@ def test_tensors_elsewhere_are_refused(gpu, which):
     b[which] = a[which]
     with pytest.raises(RuntimeError):
         scored_attn(**b)
+
+
+def test_batches_past_32_bits(gpu):
+    """Sequences 2^31 elements apart: forward, backward, rotation and norm."""
+    from gpt_from_scratch_amd import qk_norm_rotary, scored_attn
+    B, S, D, far = 2, 70, 64, 2 ** 31 + 64
+
+    def apart(n, seed):
+        big = torch.empty(far + n * S * D, dtype=torch.bfloat16, device=gpu)
+        t = big.as_strided((S, B, n, D), (n * D, far, D, 1))
+        t.copy_(randn((S, B, n, D), seed, torch.bfloat16, gpu))
+        return t
+
+    q, k, v, g = (apart(n, i) for i, n in enumerate((4, 2, 2, 4)))
+    w = randn((D,), 9, torch.float32, gpu)
+    a = torch.rand(S, D // 2, generator=torch.Generator().manual_seed(1)).to(gpu)
+
+    def call(q, k, v, g):
+        x = [t.detach().requires_grad_() for t in (q, k, v)]
+        qr, kr = qk_norm_rotary(x[0], x[1], w, w, a.cos(), a.sin())
+        o = scored_attn(qr.permute(1, 2, 0, 3), kr.permute(1, 2, 0, 3), x[2].permute(1, 2, 0, 3))
+        direct = scored_attn(*(t.permute(1, 2, 0, 3) for t in x), softcap=20.0)
+        do = g.permute(1, 2, 0, 3)
+        return (o, *torch.autograd.grad(o, x, do), direct, *torch.autograd.grad(direct, x, do))
+
+    for s, t in zip(call(q, k, v, g), call(*(t.contiguous() for t in (q, k, v, g)))):
+        assert torch.equal(s, t)
+
+
+def test_two_threads(gpu):
+    """Two host threads, each on its own stream: the bits of one after the other."""
+    import threading
+    from gpt_from_scratch_amd import decode_attn, qk_norm_rotary, scored_attn
+    a = torch.rand(300, 32, generator=torch.Generator().manual_seed(1)).to(gpu)
+    cos, sin = a.cos(), a.sin()
+    w = randn((64,), 9, torch.float32, gpu)
+    data = []
+    for i in range(2):
+        x = [randn((300, 2, n, 64), 10 * i + n, torch.bfloat16, gpu) for n in (8, 2, 2)]
+        data.append((x, documents(2, 300, "packed", i, gpu), randn((2, 8, 300, 64), 40 + i,
+                                                                     torch.bfloat16, gpu)))
+
+    def work(x, ids, do):
+        x = [t.detach().requires_grad_() for t in x]
+        q, k = qk_norm_rotary(x[0], x[1], w, w, cos, sin)
+        q, k, v = (t.permute(1, 2, 0, 3) for t in (q, k, x[2]))
+        o = scored_attn(q, k, v, document_ids=ids)
+        with torch.no_grad():
+            d = decode_attn(q[:, :, -1], k, v)
+        return (o.detach(), d, *torch.autograd.grad(o, x, do))
+
+    want = [work(*d) for d in data]
+    torch.cuda.synchronize()
+    bad = []
+
+    def run_on(i):
+        st = torch.cuda.Stream()
+        with torch.cuda.stream(st):
+            for _ in range(20):
+                got = work(*data[i])
+                st.synchronize()
+                if not all(torch.equal(s, t) for s, t in zip(got, want[i])):
+                    bad.append(i)
+
+    threads = [threading.Thread(target=run_on, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
