@@ -131,7 +131,7 @@ struct Buffers {
   int* list;       // see TileWalk
 };
 
-template <typename E, int D, bool CAP, bool BIAS>
+template <typename E, int D, bool CAP, bool BIAS, bool DOCS>
 __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Buffers& buf) {
   using L = Lay<E, D>;
   constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
@@ -148,9 +148,9 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
             b = bk / a.Hk, hk = bk % a.Hk;
   const int k0 = kt * OWN, kw = k0 + 32 * wave, krow = kw + l32;
   const bool wave_valid = kw < Sk;
-  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int* docs = DOCS ? a.docs + (int64_t)b * Sk : nullptr;
   const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
-  const int kdoc = docs && krow < Sk ? docs[krow] : 0;
+  const int kdoc = DOCS && krow < Sk ? docs[krow] : 0;
   // first query position that sees this lane's key, and the wave's first
   int qfirst = 0, wfirst = 0;
   if (a.causal) {
@@ -175,19 +175,23 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   }
 
   const int kmax = min(k0 + OWN, Sk) - 1;
-  DocRange own = {0, 0, false};
-  if (docs) own = doc_range(docs, k0, kmax - k0 + 1, lane);
+  DocRange own = {};
+  if (DOCS) own = doc_range(docs, k0, kmax - k0 + 1, lane);
   const DocTile* qtiles = a.qtiles + (int64_t)b * ((Sq + 63) / 64);
   const int nqt = (Sq + T - 1) / T;
   // first query that sees a key of the workgroup, and the first that sees all of them
   const int qlive = a.causal && k0 >= prefix ? max(k0 - a.off, 0) : 0;
   const int qfull = a.causal && kmax >= prefix ? max(kmax - a.off, 0) : 0;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const DocTile w = qtiles[t * T >> 6];
-    const bool live = (t + 1) * T > qlive && w.lo <= own.hi && w.hi >= own.lo;
-    const bool full = t * T >= qfull && (t + 1) * T <= Sq && w.lo == w.hi && own.lo == own.hi &&
-                      w.lo == own.lo && !w.pad && !own.pad;
-    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
+    if ((t + 1) * T <= qlive) return 0;
+    int f = doc_bits(qtiles[t * T >> 6], own);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int last = min(k0 + 32 * i + 31, Sk - 1);  // of block i
+      const int seen = a.causal && last >= prefix ? last - a.off : 0;  // from this query on
+      if (t * T < seen || (t + 1) * T > Sq) f &= ~(kFull << i);
+    }
+    return f;
   };
   Stage<E, D, T> qsrc, gsrc;
   qsrc.init(a.q, b, 0, a.dch, lane, wave);
@@ -197,7 +201,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
     const int q0 = (t & kTileIndex) * T;
     qsrc.base = qbase + head * a.q.sh * L::ESZ;
     gsrc.base = gbase + head * a.dout.sh * L::ESZ;
-    if (t & kPad) {
+    if (DOCS && (t & kPad)) {
       qsrc.load_padded(q0, Sq, qb, lane, wave, docs + a.off + q0);
       gsrc.load_padded(q0, Sq, gb, lane, wave, docs + a.off + q0);
     } else {
@@ -209,7 +213,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
     if (lane < T) {
       if (wave == 0) buffer_load_lds4(tile_rsrc(a.lse2 + row, nr), 4 * lane, sb);
       if (wave == 1) buffer_load_lds4(tile_rsrc(a.delta + row, nr), 4 * lane, sb + T);
-      if (wave == 2 && docs)
+      if (wave == 2 && DOCS)
         buffer_load_lds4(tile_rsrc(docs + a.off + q0, nr), 4 * lane, sb + 2 * T);
     }
   };
@@ -229,8 +233,8 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
     if (nxt >= 0) fetch(nxt, hnext, I ? Q0 : Q1, I ? G0 : G1, I ? S0 : S1);
     rd.refresh();
     const int q0 = (cur & kTileIndex) * T, p0 = a.off + q0;
-    if (wave_valid && p0 + T - 1 >= wfirst) {
-      const bool full = cur & kFull;
+    if (wave_valid && (!DOCS || (cur & kLive << wave)) && p0 + T - 1 >= wfirst) {
+      const bool full = cur & kFull << wave;
       u32x4 pb[TB][L::NG], sb[TB][L::NG];
       f32x16 ss[TB], dps[TB];
 #pragma unroll
@@ -292,7 +296,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
             const int n = 8 * (r >> 2) + (r & 3);
             if ((uint32_t)(n - lo) >= span) s[r] = dp[r] = 0.f;
           }
-          if (docs) {
+          if (DOCS) {
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
               const i32x4 d4 = *(const i32x4*)(st + 2 * T + 32 * qb + 8 * jj + 4 * g);
@@ -323,7 +327,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
   // the group's query heads one after another
   for (int first = 0; first < nqt; first += kListed) {
     TileWalk walk;
-    if (docs) {
+    if (DOCS) {
       walk.list = buf.list;
       walk.count = tile_list(buf.list, first, nqt, look);
     } else {
@@ -372,7 +376,7 @@ __device__ __forceinline__ void dkdv_item(const SAttnArgs& a, int item, const Bu
 // ---------------------------------------------------------------------------
 // dQ
 // ---------------------------------------------------------------------------
-template <typename E, int D, bool CAP, bool BIAS>
+template <typename E, int D, bool CAP, bool BIAS, bool DOCS>
 __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buffers& buf) {
   using L = Lay<E, D>;
   constexpr int OWN = 128, T = kTile<E, D>, TB = T / 32;
@@ -389,10 +393,10 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   const int h = hk * a.G + n / BHk;
   const int q0 = qt * OWN, qw = q0 + 32 * wave, qrow = qw + l32, qpos = a.off + qrow;
   const bool wave_valid = qw < Sq;
-  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int* docs = DOCS ? a.docs + (int64_t)b * Sk : nullptr;
   const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
   const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
-  const int qdoc = docs && qrow < Sq ? docs[qpos] : 0;
+  const int qdoc = DOCS && qrow < Sq ? docs[qpos] : 0;
   int klast = Sk - 1, wlast = Sk - 1;
   if (a.causal) {
     klast = min(max(qpos, prefix - 1), Sk - 1);
@@ -409,17 +413,19 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   const float ndelta = qrow < Sq ? -a.delta[row] : 0.f;
 
   const int pmin = a.off + q0, pmax = a.off + min(q0 + OWN, Sq) - 1;
-  DocRange own = {0, 0, false};
-  if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
+  DocRange own = {};
+  if (DOCS) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + 63) / 64);
   const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + T - 1) / T;
   const int kfull = a.causal ? min(max(pmin + 1, prefix), Sk) : Sk;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const DocTile w = ktiles[t * T >> 6];
-    const bool live = w.lo <= own.hi && w.hi >= own.lo;
-    const bool full = (t + 1) * T <= kfull && w.lo == w.hi && own.lo == own.hi &&
-                      w.lo == own.lo && !w.pad && !own.pad;
-    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
+    int f = doc_bits(ktiles[t * T >> 6], own);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int seen = a.causal ? max(pmin + 32 * i + 1, prefix) : Sk;  // of block i's first row
+      if ((t + 1) * T > min(seen, Sk)) f &= ~(kFull << i);
+    }
+    return f;
   };
 
   Stage<E, D, T> ksrc, vsrc;
@@ -429,14 +435,14 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   rd.init(lane);
   auto fetch = [&](int t, char* kb, char* vb, int* ib) __attribute__((always_inline)) {
     const int k0 = (t & kTileIndex) * T;
-    if (t & kPad) {
+    if (DOCS && (t & kPad)) {
       ksrc.load_padded(k0, Sk, kb, lane, wave, docs + k0);
       vsrc.load_padded(k0, Sk, vb, lane, wave, docs + k0);
     } else {
       ksrc.load(k0, Sk, kb, wave);
       vsrc.load(k0, Sk, vb, wave);
     }
-    if (docs && wave == 0 && lane < T)
+    if (DOCS && wave == 0 && lane < T)
       buffer_load_lds4(tile_rsrc(docs + k0, 4 * min(T, Sk - k0)), 4 * lane, (float*)ib);
   };
 
@@ -452,7 +458,7 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
     if (nxt >= 0) fetch(nxt, I ? K0 : K1, I ? V0 : V1, I ? I0 : I1);
     rd.refresh();
     const int k0 = (cur & kTileIndex) * T;
-    if (wave_valid && k0 <= wlast) {
+    if (wave_valid && (!DOCS || (cur & kLive << wave)) && k0 <= wlast) {
       u32x4 sb[TB][L::NG];
       f32x16 ss[TB], dps[TB];
 #pragma unroll
@@ -488,12 +494,12 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
           dp[r] *= fast_exp2(x);
           if constexpr (CAP) dp[r] *= score_slope<E, CAP>(y);
         }
-        if (!(cur & kFull)) {
+        if (!(cur & kFull << wave)) {
           const int rel = klast - k0 - 32 * kb - 4 * g;
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (8 * (r >> 2) + (r & 3) > rel) dp[r] = 0.f;
-          if (docs) {
+          if (DOCS) {
 #pragma unroll
             for (int jj = 0; jj < 4; ++jj) {
               const i32x4 d4 = *(const i32x4*)(it + 32 * kb + 8 * jj + 4 * g);
@@ -518,7 +524,7 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
   };
   for (int first = 0; first < ntiles; first += kListed) {
     TileWalk walk;
-    if (docs) {
+    if (DOCS) {
       walk.list = buf.list;
       walk.count = tile_list(buf.list, first, ntiles, look);
     } else {
@@ -558,7 +564,9 @@ __device__ __forceinline__ void dq_item(const SAttnArgs& a, int item, const Buff
 // Both kinds in one launch, so that the short items of one fill the gaps that the
 // long ones of the other leave.  Runs of 64 workgroups (whole rounds over the XCDs)
 // belong to one kind, spread evenly; each kind's own order is longest first.
-template <typename E, int D, bool CAP, bool BIAS>
+// DOCS as in the forward (B8 H12 S1024 D64 70 -> 67 us, with slopes 93 -> 86; B2 H16/4
+// S4096 D128 with a cap 665 -> 632).
+template <typename E, int D, bool CAP, bool BIAS, bool DOCS>
 __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_bwd_kernel(SAttnArgs a, int n0,
                                                                                int n1) {
   using L = Lay<E, D>;
@@ -578,9 +586,9 @@ __global__ __launch_bounds__(256, (kWavesPerSimd<E, D>)) void sattn_bwd_kernel(S
   const int item = (dkdv ? before : (int)t - before) * 64 + blockIdx.x % 64;
   if (item >= (dkdv ? n0 : n1)) return;
   if (dkdv)
-    dkdv_item<E, D, CAP, BIAS>(a, item, buf);
+    dkdv_item<E, D, CAP, BIAS, DOCS>(a, item, buf);
   else
-    dq_item<E, D, CAP, BIAS>(a, item, buf);
+    dq_item<E, D, CAP, BIAS, DOCS>(a, item, buf);
 }
 
 // The sums of split items.  Workgroups [0, n0): dV and dK of the key tiles, two
@@ -613,11 +621,11 @@ __global__ __launch_bounds__(256) void sattn_sum_kernel(SAttnArgs a, int n0) {
                    t.ss * L::ESZ, a.dch, min(32, rows - row));
 }
 
-template <typename E, int D, bool CAP, bool BIAS>
+template <typename E, int D, bool CAP, bool BIAS, bool DOCS>
 hipError_t launch_cb(const SAttnArgs& a, hipStream_t st) {
   const int kitems = (a.Sk + 127) / 128 * a.B * a.Hk, qitems = (a.Sq + 127) / 128 * a.B * a.H;
   const int n0 = kitems * a.parts, n1 = qitems * a.qparts;
-  hipLaunchKernelGGL((sattn_bwd_kernel<E, D, CAP, BIAS>), dim3(((n0 + 63) / 64 + (n1 + 63) / 64) * 64),
+  hipLaunchKernelGGL((sattn_bwd_kernel<E, D, CAP, BIAS, DOCS>), dim3(((n0 + 63) / 64 + (n1 + 63) / 64) * 64),
                      dim3(256), 0, st, a, n0, n1);
   const hipError_t e = hipGetLastError();
   const int s0 = a.parts > 1 ? 2 * kitems : 0, s1 = a.qparts > 1 ? qitems : 0;
@@ -637,10 +645,14 @@ hipError_t launch_delta(const SAttnArgs& a, hipStream_t st) {
 
 template <typename E, int D>
 hipError_t launch_d(const SAttnArgs& a, bool cap, hipStream_t st) {
-  if (cap && a.slopes) return launch_cb<E, D, true, true>(a, st);
-  if (cap) return launch_cb<E, D, true, false>(a, st);
-  if (a.slopes) return launch_cb<E, D, false, true>(a, st);
-  return launch_cb<E, D, false, false>(a, st);
+  auto run = [&](auto c, auto b) {
+    constexpr bool C = decltype(c)::value, B = decltype(b)::value;
+    return a.docs ? launch_cb<E, D, C, B, true>(a, st) : launch_cb<E, D, C, B, false>(a, st);
+  };
+  if (cap && a.slopes) return run(std::true_type{}, std::true_type{});
+  if (cap) return run(std::true_type{}, std::false_type{});
+  if (a.slopes) return run(std::false_type{}, std::true_type{});
+  return run(std::false_type{}, std::false_type{});
 }
 
 template <typename E>

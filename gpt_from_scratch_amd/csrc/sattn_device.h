@@ -296,42 +296,63 @@ struct DecodeArgs {
   float* ml;           // [B * H, splits, 2]
 };
 
-// Document ids of rows [row0, row0 + n) seen by a whole wave.
+// Document ids of up to 128 rows, by blocks of 32, seen by a whole wave: block i's range
+// in the lanes from kBlockLane[i] on (eight scalars would be spilled for the length of
+// a kernel that needs them now and then); bit i of pad: a negative id in block i.
 struct DocRange {
-  int lo, hi;
-  bool pad;
+  int lo, hi, pad;
+  static constexpr int kBlockLane[4] = {0, 32, 16, 48};
+  __device__ __forceinline__ int block_lo(int i) const {
+    return __builtin_amdgcn_readlane(lo, kBlockLane[i]);
+  }
+  __device__ __forceinline__ int block_hi(int i) const {
+    return __builtin_amdgcn_readlane(hi, kBlockLane[i]);
+  }
 };
 __device__ __forceinline__ DocRange doc_range(const int* ids, int row0, int n, int lane) {
-  int lo = 0x7fffffff, hi = -1, pad = 0;
-  for (int i = lane; i < n; i += 64) {
-    const int d = ids[row0 + i];
-    if (d < 0) {
-      pad = 1;
-    } else {
-      lo = min(lo, d);
-      hi = max(hi, d);
-    }
-  }
+  int lo[2], hi[2], pad = 0;
 #pragma unroll
-  for (int m = 32; m; m >>= 1) {
-    lo = min(lo, __shfl_xor(lo, m, 64));
-    hi = max(hi, __shfl_xor(hi, m, 64));
+  for (int j = 0; j < 2; ++j) {
+    const int i = lane + 64 * j, d = i < n ? ids[row0 + i] : 0x7fffffff;
+    const bool some = i < n && d >= 0;
+    lo[j] = some ? d : 0x7fffffff;
+    hi[j] = some ? d : -1;
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+      lo[j] = min(lo[j], __shfl_xor(lo[j], m, 64));
+      hi[j] = max(hi[j], __shfl_xor(hi[j], m, 64));
+    }
+    const uint64_t p = __ballot(d < 0);
+    pad |= ((uint32_t)p ? 1 << 2 * j : 0) | (p >> 32 ? 2 << 2 * j : 0);
   }
-  DocRange r;
-  r.lo = __builtin_amdgcn_readfirstlane(lo);
-  r.hi = __builtin_amdgcn_readfirstlane(hi);
-  r.pad = __any(pad);
-  return r;
+  const bool second = lane & 16;
+  return {second ? lo[1] : lo[0], second ? hi[1] : hi[0], pad};
 }
 
 // The streamed tiles a workgroup has to visit, in order.  Without documents a range;
 // with them a list in LDS, built 64 tiles at a time (lane t looks at one tile, a
 // ballot gives the live ones their places), at most kListed tiles of the sequence in
-// one list.  An entry is a tile's index with kFull (every pair visible: no mask) and
-// kPad (rows of negative document id in it).  The walk over it, `heads` times for dK / dV, takes the entries part,
+// one list.  An entry is a tile's index; for each block of 32 of the workgroup's rows
+// kLive (it shares a document with the tile: the others' waves have nothing to do)
+// and kFull (every pair visible: no mask); and kPad (rows of negative document id in
+// it).  The walk over it, `heads` times for dK / dV, takes the entries part,
 // part + parts, ...: equal shares whatever the mask.
-constexpr int kFull = 1 << 30, kPad = 1 << 29, kTileIndex = kPad - 1;
+constexpr int kTileIndex = (1 << 20) - 1, kFull = 1 << 20, kLive = 1 << 24, kPad = 1 << 29;
+constexpr int kBlocks = 15;  // all four of either
 constexpr int kListed = 512;
+
+// kLive, kPad and, as far as documents go, kFull of a tile.
+__device__ __forceinline__ int doc_bits(const DocTile& w, const DocRange& own) {
+  int f = w.pad ? kPad : 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int lo = own.block_lo(i), hi = own.block_hi(i);
+    if (w.lo <= hi && w.hi >= lo) f |= kLive << i;
+    if (w.lo == w.hi && w.lo == lo && w.lo == hi && !w.pad && !(own.pad >> i & 1))
+      f |= kFull << i;
+  }
+  return f;
+}
 
 struct TileWalk {
   const int* list;                 // null: tiles [lo, lo + count), full in [f0, f1)
@@ -341,7 +362,7 @@ struct TileWalk {
     if (head >= hend) return -1;
     if (list) return __builtin_amdgcn_readfirstlane(list[at]);
     const int t = lo + at;
-    return t >= f0 && t < f1 ? t | kFull : t;
+    return t | kLive * kBlocks | (t >= f0 && t < f1 ? kFull * kBlocks : 0);
   }
   __device__ __forceinline__ void step(int n) {
     at += n;
@@ -359,7 +380,8 @@ struct TileWalk {
   }
 };
 
-// Tiles [first, first + kListed) of n; `look` says of one: bit 0 live, kFull, kPad.
+// Tiles [first, first + kListed) of n; `look` gives an entry's bits, kLive for none if
+// the tile is not visited.
 // Ends with a barrier.
 template <typename F>
 __device__ __forceinline__ int tile_list(int* list, int first, int n, F look) {
@@ -367,9 +389,9 @@ __device__ __forceinline__ int tile_list(int* list, int first, int n, F look) {
   int count = 0;
   for (int t0 = first; t0 < end; t0 += 64) {
     const int f = t0 + lane < end ? look(t0 + lane) : 0;
-    const uint64_t live = __ballot(f & 1);
-    if ((f & 1) && threadIdx.x < 64)
-      list[count + __popcll(live & ((1ull << lane) - 1))] = (t0 + lane) | (f & (kFull | kPad));
+    const uint64_t live = __ballot(f & kLive * kBlocks);
+    if ((f & kLive * kBlocks) && threadIdx.x < 64)
+      list[count + __popcll(live & ((1ull << lane) - 1))] = (t0 + lane) | f;
     count += __popcll(live);
   }
   __syncthreads();

@@ -41,7 +41,8 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* docs, DocTile
   const int per = key ? nk : nq, b = (int)(j / per), t = (int)(j % per);
   const int off = key ? 0 : Sk - Sq, rows = key ? Sk : Sq;
   const DocRange r = doc_range(docs + (int64_t)b * Sk, off + 64 * t, min(64, rows - 64 * t), lane);
-  if (lane == 0) out[i] = DocTile{r.lo, r.hi, r.pad, 0};
+  const int lo[2] = {r.block_lo(0), r.block_lo(1)}, hi[2] = {r.block_hi(0), r.block_hi(1)};
+  if (lane == 0) out[i] = DocTile{min(lo[0], lo[1]), max(hi[0], hi[1]), r.pad != 0, 0};
 }
 
 // A wave's O (normalised) and lse.  A row without a visible key: O = 0, lse = -inf.
@@ -63,14 +64,19 @@ __device__ __forceinline__ void finish_rows(const SAttnArgs& a, int b, int h, in
 
 constexpr float kSlack = 8.f;  // log2 units a score may exceed the running reference by
 
-// Waves per SIMD the register budget is held to.
-template <typename E, int D, bool BIAS>
-constexpr int kFwdWaves = Lay<E, D>::RB > 256 ? 1 : Lay<E, D>::RB > 128 ? 2 : BIAS ? 3 : 4;
+// Waves per SIMD the register budget is held to.  Documents: one fewer, or the mask's ids
+// cost spills in every step (B8 H24 S1024 D64, 4 documents: 46 us against 30.5).
+template <typename E, int D, bool BIAS, bool DOCS, int KS>
+constexpr int kFwdWaves = Lay<E, D>::RB > 256   ? 1
+                          : Lay<E, D>::RB > 128 ? 2
+                                                : (BIAS ? 3 : 4) - (DOCS && KS == 1 ? 1 : 0);
 
+// DOCS: with document ids.  Without, the code for them is not there at all: 2 to 8% (B8 H12
+// S1024 D64 24.3 -> 22.6 us, B2 H16/4 S2048 D128 53.5 -> 51.9).
 // KS = 2: a wave takes one 32-key block of each tile instead of both, two waves share
 // 32 query rows and merge at the end, and a workgroup owns 64 rows (see key_split).
-template <typename E, int D, bool CAP, bool BIAS, int KS>
-__global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel(SAttnArgs a) {
+template <typename E, int D, bool CAP, bool BIAS, bool DOCS, int KS>
+__global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS, DOCS, KS>)) void sattn_fwd_kernel(SAttnArgs a) {
   using L = Lay<E, D>;
   constexpr int BQ = 128 / KS, BK = 64, NB = 2 / KS;
   __shared__ __attribute__((aligned(16))) char K0[BK * L::RB];
@@ -96,7 +102,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   const int q0 = qt * BQ, qw = q0 + 32 * (wave / KS), qrow = qw + l32, qpos = a.off + qrow;
   const int slice = KS == 1 ? 0 : wave & 1;
   const bool wave_valid = qw < Sq;
-  const int* docs = a.docs ? a.docs + (int64_t)b * Sk : nullptr;
+  const int* docs = DOCS ? a.docs + (int64_t)b * Sk : nullptr;
   const int prefix = a.prefix ? max(a.prefix[b], 0) : 0;
   const float slope2 = BIAS ? a.slopes[h] * kLog2e : 0.f;
 
@@ -106,7 +112,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   for (int ks = 0; ks < L::KS; ++ks)
     qf[ks] = qrow < Sq && 2 * ks + g < a.dch ? *(const u32x4*)(qp + 16 * (2 * ks + g))
                                               : u32x4{0, 0, 0, 0};
-  const int qdoc = docs && qrow < Sq ? docs[qpos] : 0;
+  const int qdoc = DOCS && qrow < Sq ? docs[qpos] : 0;
   // last key that position and sequence end leave visible; none for padding
   int klast = Sk - 1, wlast = Sk - 1;
   if (a.causal) {
@@ -116,18 +122,20 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   if (qdoc < 0) klast = -1;
 
   const int pmin = a.off + q0, pmax = a.off + min(q0 + BQ, Sq) - 1;
-  DocRange own = {0, 0, false};
-  if (docs) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
+  DocRange own = {};
+  if (DOCS) own = doc_range(docs, pmin, pmax - pmin + 1, lane);
   const DocTile* ktiles = a.ktiles + (int64_t)b * ((Sk + BK - 1) / BK);
   const int kend = a.causal ? min(max(pmax + 1, prefix), Sk) : Sk, ntiles = (kend + BK - 1) / BK;
   // full: all keys before every query of the workgroup, or in the prefix
   const int kfull = a.causal ? min(max(pmin + 1, prefix), Sk) : Sk;
   auto look = [&](int t) __attribute__((always_inline)) {
-    const DocTile w = ktiles[t];
-    const bool live = w.lo <= own.hi && w.hi >= own.lo;
-    const bool full = (t + 1) * BK <= kfull && w.lo == w.hi && own.lo == own.hi &&
-                      w.lo == own.lo && !w.pad && !own.pad;
-    return (live ? 1 : 0) | (full ? kFull : 0) | (w.pad ? kPad : 0);
+    int f = doc_bits(ktiles[t], own);
+#pragma unroll
+    for (int i = 0; i < 4 / KS; ++i) {
+      const int seen = a.causal ? max(pmin + 32 * i + 1, prefix) : Sk;  // of block i's first row
+      if ((t + 1) * BK > min(seen, Sk)) f &= ~(kFull << i);
+    }
+    return f;
   };
 
   Stage<E, D, BK> ksrc, vsrc;
@@ -138,14 +146,14 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
 
   auto fetch = [&](int t, char* kb, char* vb, int* ib) __attribute__((always_inline)) {
     const int k0 = (t & kTileIndex) * BK;
-    if (t & kPad) {
+    if (DOCS && (t & kPad)) {
       ksrc.load_padded(k0, Sk, kb, lane, wave, docs + k0);
       vsrc.load_padded(k0, Sk, vb, lane, wave, docs + k0);
     } else {
       ksrc.load(k0, Sk, kb, wave);
       vsrc.load(k0, Sk, vb, wave);
     }
-    if (docs && wave == 0)
+    if (DOCS && wave == 0)
       buffer_load_lds4(tile_rsrc(docs + k0, 4 * min(BK, Sk - k0)), 4 * lane, (float*)ib);
   };
 
@@ -170,7 +178,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
     if (nxt >= 0) fetch(nxt, I ? K0 : K1, I ? V0 : V1, I ? I0 : I1);
     rd.refresh();
     const int k0 = (cur & kTileIndex) * BK + 32 * slice;  // the wave's first key
-    if (wave_valid && k0 <= wlast) {
+    if (wave_valid && (!DOCS || (cur & kLive << wave / KS)) && k0 <= wlast) {
       f32x16 s[NB];
 #pragma unroll
       for (int ks = 0; ks < L::KS; ++ks)
@@ -206,14 +214,14 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
                   s[kb][r] * a.sc.f);
         }
       }
-      if (!(cur & kFull)) {
+      if (!(cur & kFull << wave / KS)) {
         const int rel = klast - k0 - 4 * g;
 #pragma unroll
         for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
           for (int r = 0; r < 16; ++r)
             if (32 * kb + 8 * (r >> 2) + (r & 3) > rel) s[kb][r] = -INFINITY;
-        if (docs) {
+        if (DOCS) {
 #pragma unroll
           for (int kb = 0; kb < NB; ++kb)
 #pragma unroll
@@ -284,7 +292,7 @@ __global__ __launch_bounds__(256, (kFwdWaves<E, D, BIAS>)) void sattn_fwd_kernel
   };
   for (int first = 0; first < ntiles; first += kListed) {
     TileWalk walk;
-    if (docs) {
+    if (DOCS) {
       walk.list = list;
       walk.count = tile_list(list, first, ntiles, look);
     } else {
@@ -400,14 +408,16 @@ int fwd_parts(const SAttnArgs& a, bool f32) {
 template <typename E, int D, int KS>
 hipError_t launch_k(const SAttnArgs& a, bool cap, hipStream_t st) {
   const dim3 grid((a.Sq + 128 / KS - 1) / (128 / KS) * a.B * a.H * a.parts), block(256);
-  if (cap && a.slopes)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, true, KS>), grid, block, 0, st, a);
-  else if (cap)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, true, false, KS>), grid, block, 0, st, a);
-  else if (a.slopes)
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, true, KS>), grid, block, 0, st, a);
-  else
-    hipLaunchKernelGGL((sattn_fwd_kernel<E, D, false, false, KS>), grid, block, 0, st, a);
+  const bool docs = a.docs;
+  auto run = [&](auto c, auto b) {
+    constexpr bool C = decltype(c)::value, B = decltype(b)::value;
+    if (docs) hipLaunchKernelGGL((sattn_fwd_kernel<E, D, C, B, true, KS>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((sattn_fwd_kernel<E, D, C, B, false, KS>), grid, block, 0, st, a);
+  };
+  if (cap && a.slopes) run(std::true_type{}, std::true_type{});
+  else if (cap) run(std::true_type{}, std::false_type{});
+  else if (a.slopes) run(std::false_type{}, std::true_type{});
+  else run(std::false_type{}, std::false_type{});
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess || a.parts == 1) return e;
   hipLaunchKernelGGL((sattn_join_kernel<E, D>), dim3((a.Sq + 127) / 128 * a.B * a.H), block, 0, st,
