@@ -19,7 +19,7 @@
 //
 // Bound by a step's latency (read, product, exponential, product) at two waves per
 // SIMD: causal B2 H16/4 S4096 D128 540-580 us (590-640 TFLOP/s counting 5 products),
-// B8 H12 S1024 D64 with slopes 88 us, fp32 B2 H12 S1000 D64 with a prefix 144 us.
+// B8 H12 S1024 D64 with slopes 81 us, fp32 B2 H12 S1000 D64 with a prefix 144 us.
 //
 // delta subtracts from dP what O says, so O's rounding would reach every dz of a
 // row: the forward keeps what the rounding left (olo), and delta is as exact as fp32

@@ -29,7 +29,10 @@ struct Elem {  // 16-bit types
   static __device__ __forceinline__ f32x16 mfma(u32x4 a, u32x4 b, f32x16 c) {
     return E::mfma(a, b, c);
   }
-  // Operand of k-group n from a 32x32 accumulator (rows 16n .. 16n + 15).
+  // Operand of k-group n from a 32x32 accumulator (rows 16n .. 16n + 15).  The one
+  // rounding of P (and of dS in the backward): the matrix cores take 16-bit operands
+  // at sixteen times the fp32 rate.  P is summed before it where lse is a result,
+  // after it in decoding, where the sum only divides O.
   static __device__ __forceinline__ u32x4 operand(const f32x16& s, int n) {
     u32x4 w;
 #pragma unroll

@@ -5,7 +5,7 @@
 // Bound by the matrix cores for plain scores; a cap adds two transcendentals per
 // score to the softmax's one, which take longer than the score's products.  Causal
 // B2 H16/4 S4096 D128 141-145 us (950-975 TFLOP/s); B1 H32/8 S4096 D128 with a cap
-// 172 us; B8 H12 S1024 D64 with slopes 29 us; fp32 B2 H12 S1000 D64, prefix 47 us.
+// 168 us; B8 H12 S1024 D64 with slopes 28 us; fp32 B2 H12 S1000 D64, prefix 46 us.
 //
 // Work decomposition, as in attn_fwd.hip: a workgroup (4 waves) owns 128 query
 // rows of one head, wave w rows [32w, 32w + 32); S^T = K Q^T and O^T = V^T P^T
